@@ -221,6 +221,79 @@ uint64_t tffn_session_launch_count(const tffn_session* s);
 /* the stream the session launches on (a cudaStream_t) */
 void* tffn_session_stream(const tffn_session* s);
 
+/* ---- training operators ------------------------------------------------------------------ */
+/* What a trainer of expert deltas needs of the frozen base next to tffn_expert_forward: norms and attention in both
+ * directions (the reference's trainer leaves the attention Jacobian out, trainer/src/model/qwen.cu:483-583, and
+ * materialises its probabilities, :391-413) and the loss on sampled tokens.
+ *
+ * Every tensor is a DEVICE pointer on `device`, `stream` a cudaStream_t of that device (NULL: its default stream). The
+ * calls enqueue their kernels and return; they allocate nothing, wait for nothing, keep nothing, may be captured into a
+ * CUDA graph (the first call of an operator on a device looks its kernels up and belongs outside of a capture), and leave the calling
+ * thread's current device as it was. A workspace is the caller's and may be reused as soon as the stream has passed the call; calls
+ * that can overlap, replayed graphs included, need workspaces of their own. Equal inputs give equal bits: no sum depends on timing.
+ * Arguments are checked before anything is enqueued: TFFN_ERR_INVALID, TFFN_ERR_UNSUPPORTED. What only the device can
+ * see (a wait that ran out) is left in a status word per device: tffn_train_status. */
+enum { TFFN_DTYPE_BF16 = 0, TFFN_DTYPE_F32 = 1 };
+enum { TFFN_NORM_RMS = 0, TFFN_NORM_LAYER = 1 };
+
+/* Rows of `width` (1 .. 16384) contiguous elements: y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ * TFFN_NORM_RMS has mean = 0 and no bias (bias and mean must be NULL; trainer/src/backend/cuda_ops.cu:144-170). dtype is that of x,
+ * weight, bias and y; mean and rstd are fp32 [rows] and may be NULL. y may be x. Computed in fp32, rounded once. */
+int tffn_norm_forward(int device, int kind, int dtype, const void* x, const void* weight, const void* bias, int64_t rows, int width, float eps,
+                      void* y, float* mean, float* rstd, void* stream);
+/* bytes tffn_norm_backward needs for dweight and dbias */
+int64_t tffn_norm_backward_workspace(int64_t rows, int width);
+/* With n = (x - mean) * rstd and g = dy * weight: dx = rstd * (g - n * mean(g * n) - mean(g)) + skip (the last mean for the layer norm
+ * only), dweight = sum of dy * n and dbias = sum of dy over the rows, both fp32 [width] and overwritten (trainer/src/backend/cuda_ops.cu:172-225).
+ * skip (the gradient that passes the norm by on the residual stream), dweight and dbias may be NULL; without dweight and dbias no
+ * workspace is needed. dx may be dy, x or skip. workspace: 16-byte aligned. */
+int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                       const void* skip, int64_t rows, int width, void* dx, float* dweight, float* dbias, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
+/* Attention of packed sequences in bf16. Sequence i has the rows cu_q[i] .. cu_q[i + 1] of q and out and cu_k[i] .. cu_k[i + 1] of k and v
+ * (device int32 [n_seqs + 1], ascending); rows outside are neither read into a result nor written. A row holds its heads one after the
+ * other (head_dim elements each, a multiple of 8 up to 128); rows are *_stride elements apart (multiples of 8, pointers 16-byte aligned), so
+ * q, k and v may be parts of one projection's output. Query heads share kv heads in groups of heads / kv_heads. The queries of a
+ * sequence are its last positions: query j has position len_k - len_q + j, and with `causal` it sees the keys up to its own position
+ * (none, if that is negative), with chunk > 0 (causal only) no key before position / chunk * chunk. A query that sees no key has
+ * out = 0, lse = -inf and no gradient. Values inside a sequence have to be finite. max_q and max_k bound the lengths (rows beyond are not
+ * computed); scale > 0. */
+typedef struct tffn_attention {
+    int32_t n_seqs, heads, kv_heads, head_dim, max_q, max_k, causal, chunk;
+    int64_t rows_q, rows_k; /* rows of the buffers */
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    float scale;
+} tffn_attention;
+/* out = softmax(scale * q k^T) v and lse = log of the softmax's denominators, fp32 [heads][rows_q] (may be NULL when no gradient
+ * follows). The weights enter their product with v as bf16; scores, sums and lse are fp32. */
+int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k, const void* v,
+                           void* out, float* lse, void* stream);
+int64_t tffn_attention_backward_workspace(const tffn_attention* a);
+/* Gradients of q, k and v from that of out (stride of out), with what the forward call left in out and lse; dq, dk and dv have the
+ * strides of q, k and v and are overwritten. The probabilities are formed again. workspace: 16-byte aligned. */
+int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k, const void* v,
+                            const void* out, const float* lse, const void* d_out, void* dq, void* dk, void* dv, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/* logprob[r] = log softmax(logits[r])[targets[r]], fp32; 0 where the target is not in 0 .. vocab - 1. logits: dtype [rows][vocab], rows
+ * row_stride elements apart (0: vocab). What a policy sampled with, or a reference model says of the same tokens. */
+int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, int64_t rows, int vocab, float* logprob,
+                        void* stream);
+/* The clipped policy loss with a KL term, and its gradient, in one pass over the logits. Per row, with lp the target's log-probability:
+ *   ratio = exp(lp - old_logprob), gain = min(ratio * advantage, clip(ratio, 1 - clip_low, 1 + clip_high) * advantage)
+ *   kl = exp(ref_logprob - lp) - (ref_logprob - lp) - 1        (0 with ref_logprob NULL)
+ *   row_loss = weight * (kl_coef * kl - gain), loss = sum of row_loss
+ * and d_logits = the gradient of loss (0 through the clipped branch; on a tie through the other one), dtype, row_stride apart; it may be
+ * logits itself. weight [rows] carries the mask and the normalisation (NULL: 1). A row of weight 0, or whose target is not in the vocabulary,
+ * is not read: its gradient, loss, logprob and kl are 0. loss [1] (needs row_loss), row_loss, logprob, kl [rows] and d_logits may be NULL. Masked
+ * vocabulary entries (-inf or the type's lowest value) weigh nothing. Rows of up to 1.7 MB (TFFN_ERR_UNSUPPORTED beyond). */
+int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, const float* old_logprob,
+                     const float* ref_logprob, const float* advantage, const float* weight, int64_t rows, int vocab, float clip_low, float clip_high,
+                     float kl_coef, float* loss, float* row_loss, float* logprob, float* kl, void* d_logits, void* stream);
+/* waits for the device and returns what the bounded waits of the training operators have reported on it so far (0: nothing) */
+int tffn_train_status(int device);
+
 /* ---- kernel-level entry points used by the tests ---------------------------------------- */
 /* out[T,N] = X[T,K] * W[N,K]^T on the tensor-core GEMM of the batched path (bf16 bits in,
  * fp32 out, host pointers); splits = 0 lets the launcher choose the K split.

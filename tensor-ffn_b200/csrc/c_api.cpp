@@ -3,6 +3,8 @@
 #include "../../include/tffn.h"
 #include "../../include/tffn_diag.h"
 #include "engine.h"
+#include "train.h"
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <vector>
@@ -421,6 +423,254 @@ int tffn_session_status(tffn_session* s) {
 }
 uint64_t tffn_session_launch_count(const tffn_session* s) { return s ? s->s->launch_count() : 0; }
 void* tffn_session_stream(const tffn_session* s) { return s ? (void*)s->s->stream() : nullptr; }
+
+// ---- training operators: arguments, the device for the length of the call, the launch
+namespace {
+
+struct OnDevice {
+    int before = -1, num_sms = 0;
+    explicit OnDevice(int device) {
+        int n = 0;
+        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+            cudaGetLastError();
+            throw Error(kErrCuda, "no CUDA device is available");
+        }
+        need(device >= 0 && device < n, "no such device");
+        TFFN_CUDA(cudaGetDevice(&before));
+        TFFN_CUDA(cudaSetDevice(device));
+        const cudaError_t e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
+        if (e != cudaSuccess) {
+            cudaSetDevice(before);
+            cuda_check(e, "cudaDeviceGetAttribute", __FILE__, __LINE__);
+        }
+    }
+    ~OnDevice() { cudaSetDevice(before); }
+    OnDevice(const OnDevice&) = delete;
+};
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+int* status_word(int device) {
+    int* p = train_status_word(device);
+    if (!p) throw Error(kErrCuda, "the training operators' status word is not available on this device");
+    return p;
+}
+NormCall norm_call(int kind, int dtype, const void* x, const void* weight, int64_t rows, int width) {
+    need(kind == TFFN_NORM_RMS || kind == TFFN_NORM_LAYER, "unknown norm kind");
+    need(dtype == TFFN_DTYPE_BF16 || dtype == TFFN_DTYPE_F32, "unknown dtype");
+    need(rows >= 0 && width > 0 && weight && (x || rows == 0), "bad norm arguments");
+    if (width > kNormMaxWidth) throw Error(kErrUnsupported, "norm rows of more than 16384 elements");
+    if (rows > (int64_t)1 << 31) throw Error(kErrUnsupported, "norm of more than 2^31 rows");
+    NormCall c;
+    memset(&c, 0, sizeof c);
+    c.layer = kind == TFFN_NORM_LAYER;
+    c.f32 = dtype == TFFN_DTYPE_F32;
+    c.x = x;
+    c.weight = weight;
+    c.rows = rows;
+    c.width = width;
+    return c;
+}
+void need_elements(int dtype, std::initializer_list<const void*> tensors) {
+    for (const void* t : tensors) need(aligned(t, dtype == TFFN_DTYPE_F32 ? 4 : 2), "a tensor is not aligned to its elements");
+}
+AttnCall attn_call(const tffn_attention* a) {
+    need(a, "NULL attention");
+    need(a->n_seqs >= 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->head_dim > 0, "bad attention heads or sequences");
+    need(a->max_q >= 0 && a->max_k >= 0 && a->rows_q >= 0 && a->rows_k >= 0, "negative attention lengths or rows");
+    need(std::isfinite(a->scale) && a->scale > 0.f, "the attention scale must be positive");
+    need(a->chunk >= 0 && (a->chunk == 0 || a->causal), "chunks need a causal mask");
+    if (a->head_dim % 8 || a->head_dim > 128) throw Error(kErrUnsupported, "attention heads must be a multiple of 8 wide, at most 128");
+    if (a->heads > 65535 || a->rows_q > INT32_MAX || a->rows_k > INT32_MAX) throw Error(kErrUnsupported, "more than 65535 heads or 2^31 rows");
+    const int64_t q = (int64_t)a->heads * a->head_dim, k = (int64_t)a->kv_heads * a->head_dim;
+    need(a->q_stride >= q && a->out_stride >= q && a->k_stride >= k && a->v_stride >= k, "an attention row stride is shorter than its row");
+    need(a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0 && a->out_stride % 8 == 0, "attention row strides must be multiples of 8 elements");
+    AttnCall c;
+    memset(&c, 0, sizeof c);
+    c.n_seqs = a->n_seqs;
+    c.heads = a->heads;
+    c.kv_heads = a->kv_heads;
+    c.hd = a->head_dim;
+    c.rows_q = a->rows_q;
+    c.rows_k = a->rows_k;
+    c.max_q = (int)std::min<int64_t>(a->max_q, a->rows_q);
+    c.max_k = (int)std::min<int64_t>(a->max_k, a->rows_k);
+    c.q_stride = a->q_stride;
+    c.k_stride = a->k_stride;
+    c.v_stride = a->v_stride;
+    c.out_stride = a->out_stride;
+    c.scale = a->scale;
+    c.causal = a->causal != 0;
+    c.chunk = a->chunk;
+    return c;
+}
+void need_rows(std::initializer_list<const void*> tensors, int64_t rows) {
+    for (const void* t : tensors) need((t || rows == 0) && aligned(t, 16), "a tensor is NULL or not 16-byte aligned");
+}
+LossCall loss_call(int dtype, const void* logits, int64_t row_stride, const int32_t* targets, int64_t rows, int vocab) {
+    need(dtype == TFFN_DTYPE_BF16 || dtype == TFFN_DTYPE_F32, "unknown dtype");
+    need(rows >= 0 && vocab > 0 && (row_stride == 0 || row_stride >= vocab), "bad logits shape");
+    need(rows == 0 || (logits && targets), "NULL logits or targets");
+    need_elements(dtype, {logits});
+    if (rows > (int64_t)1 << 27) throw Error(kErrUnsupported, "more than 2^27 rows of logits");
+    LossCall c;
+    memset(&c, 0, sizeof c);
+    c.f32 = dtype == TFFN_DTYPE_F32;
+    c.logits = logits;
+    c.rows = rows;
+    c.stride = row_stride ? row_stride : vocab;
+    c.vocab = vocab;
+    c.targets = targets;
+    return c;
+}
+
+}  // namespace
+
+int tffn_norm_forward(int device, int kind, int dtype, const void* x, const void* weight, const void* bias, int64_t rows, int width, float eps, void* y,
+                      float* mean, float* rstd, void* stream) {
+    return guard([&] {
+        NormCall c = norm_call(kind, dtype, x, weight, rows, width);
+        need(std::isfinite(eps) && eps >= 0.f, "bad norm eps");
+        need(y || rows == 0, "NULL output");
+        need(c.layer ? bias != nullptr : !bias && !mean, "the layer norm needs a bias; the RMS norm has no bias and no mean");
+        need_elements(dtype, {x, weight, bias, y});
+        c.bias = bias;
+        c.eps = eps;
+        c.y = y;
+        c.mean = mean;
+        c.rstd = rstd;
+        OnDevice on(device);
+        check_launch(launch_norm_forward(c, on.num_sms, (cudaStream_t)stream), "norm forward");
+    });
+}
+int64_t tffn_norm_backward_workspace(int64_t rows, int width) {
+    int64_t bytes = 0;
+    const int rc = guard([&] {
+        need(rows >= 0 && width > 0 && width <= kNormMaxWidth, "bad norm shape");
+        bytes = norm_workspace_floats(rows, width) * 4;
+    });
+    return rc < 0 ? rc : bytes;
+}
+int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                       const void* skip, int64_t rows, int width, void* dx, float* dweight, float* dbias, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+    return guard([&] {
+        NormCall c = norm_call(kind, dtype, x, weight, rows, width);
+        need(rows == 0 || (dy && dx && rstd), "NULL gradient or rstd");
+        need(c.layer ? mean || rows == 0 : !mean && !dbias, "the layer norm needs its mean; the RMS norm has no mean and no bias");
+        need_elements(dtype, {dy, x, weight, skip, dx});
+        if (dweight || dbias)
+            need(rows == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= norm_workspace_floats(rows, width) * 4),
+                 "norm workspace missing, not 16-byte aligned or too small");
+        c.dy = dy;
+        c.mean = const_cast<float*>(mean);
+        c.rstd = const_cast<float*>(rstd);
+        c.skip = skip;
+        c.dx = dx;
+        c.dweight = dweight;
+        c.dbias = dbias;
+        c.workspace = (float*)workspace;
+        OnDevice on(device);
+        check_launch(launch_norm_backward(c, on.num_sms, (cudaStream_t)stream), "norm backward");
+    });
+}
+int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k, const void* v,
+                           void* out, float* lse, void* stream) {
+    return guard([&] {
+        AttnCall c = attn_call(a);
+        need(cu_q && cu_k, "NULL offsets");
+        need_rows({q, out}, c.rows_q);
+        need_rows({k, v}, c.rows_k);
+        c.cu_q = cu_q;
+        c.cu_k = cu_k;
+        c.q = (const bf16*)q;
+        c.k = (const bf16*)k;
+        c.v = (const bf16*)v;
+        c.out = (bf16*)out;
+        c.lse = lse;
+        OnDevice on(device);
+        c.status = status_word(device);
+        check_launch(launch_attention_train_forward(c, (cudaStream_t)stream), "attention forward");
+    });
+}
+int64_t tffn_attention_backward_workspace(const tffn_attention* a) {
+    int64_t bytes = 0;
+    const int rc = guard([&] { bytes = attention_workspace_bytes(attn_call(a)); });
+    return rc < 0 ? rc : bytes;
+}
+int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k, const void* v,
+                            const void* out, const float* lse, const void* d_out, void* dq, void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+    return guard([&] {
+        AttnCall c = attn_call(a);
+        need(cu_q && cu_k, "NULL offsets");
+        need_rows({q, out, d_out, dq}, c.rows_q);
+        need_rows({k, v, dk, dv}, c.rows_k);
+        need(lse || c.rows_q == 0, "NULL lse");
+        const int64_t bytes = attention_workspace_bytes(c);
+        need(bytes == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= bytes), "attention workspace missing, not 16-byte aligned or too small");
+        c.cu_q = cu_q;
+        c.cu_k = cu_k;
+        c.q = (const bf16*)q;
+        c.k = (const bf16*)k;
+        c.v = (const bf16*)v;
+        c.out = (bf16*)const_cast<void*>(out);
+        c.lse = const_cast<float*>(lse);
+        c.d_out = (const bf16*)d_out;
+        c.dq = (bf16*)dq;
+        c.dk = (bf16*)dk;
+        c.dv = (bf16*)dv;
+        c.workspace = workspace;
+        OnDevice on(device);
+        c.status = status_word(device);
+        check_launch(launch_attention_train_backward(c, (cudaStream_t)stream), "attention backward");
+    });
+}
+int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, int64_t rows, int vocab, float* logprob,
+                        void* stream) {
+    return guard([&] {
+        LossCall c = loss_call(dtype, logits, row_stride, targets, rows, vocab);
+        need(logprob || rows == 0, "NULL output");
+        c.logprob = logprob;
+        OnDevice on(device);
+        check_launch(launch_token_logprobs(c, on.num_sms, (cudaStream_t)stream), "token log-probabilities");
+    });
+}
+int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, const float* old_logprob,
+                     const float* ref_logprob, const float* advantage, const float* weight, int64_t rows, int vocab, float clip_low, float clip_high,
+                     float kl_coef, float* loss, float* row_loss, float* logprob, float* kl, void* d_logits, void* stream) {
+    return guard([&] {
+        LossCall c = loss_call(dtype, logits, row_stride, targets, rows, vocab);
+        need(rows == 0 || (old_logprob && advantage), "NULL old_logprob or advantage");
+        need(!loss || row_loss || rows == 0, "loss needs row_loss");
+        need(clip_low >= 0.f && clip_low <= 1.f && clip_high >= 0.f && std::isfinite(clip_high) && std::isfinite(kl_coef), "bad clip range or KL coefficient");
+        need_elements(dtype, {d_logits});
+        if (!policy_loss_supported(c.f32, vocab)) throw Error(kErrUnsupported, "rows of logits of more than 1.7 MB");
+        c.old_logprob = old_logprob;
+        c.ref_logprob = ref_logprob;
+        c.advantage = advantage;
+        c.weight = weight;
+        c.clip_low = clip_low;
+        c.clip_high = clip_high;
+        c.kl_coef = kl_coef;
+        c.loss = loss;
+        c.row_loss = row_loss;
+        c.logprob = logprob;
+        c.kl = kl;
+        c.d_logits = d_logits;
+        OnDevice on(device);
+        c.status = status_word(device);
+        check_launch(launch_policy_loss(c, on.num_sms, (cudaStream_t)stream), "policy loss");
+    });
+}
+int tffn_train_status(int device) {
+    int st = 0;
+    const int rc = guard([&] {
+        OnDevice on(device);
+        int* word = status_word(device);
+        TFFN_CUDA(cudaDeviceSynchronize());
+        TFFN_CUDA(cudaMemcpy(&st, word, 4, cudaMemcpyDeviceToHost));
+    });
+    return rc < 0 ? rc : st;
+}
 
 int tffn_op_gemm(int device, const uint16_t* X, const uint16_t* W, float* out, int T, int N, int K, int splits) {
     return tffn_op_gemm_trace(device, X, W, out, T, N, K, splits, nullptr, 0);

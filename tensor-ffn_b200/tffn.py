@@ -39,12 +39,19 @@ class Config(ctypes.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class AttentionShape(ctypes.Structure):
+    """tffn_attention: sequences, heads, mask and row strides of a training attention call"""
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_seqs", "heads", "kv_heads", "head_dim", "max_q", "max_k", "causal", "chunk")] + \
+               [(n, ctypes.c_int64) for n in ("rows_q", "rows_k", "q_stride", "k_stride", "v_stride", "out_stride")] + \
+               [("scale", ctypes.c_float)]
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(f"{LIB_PATH} is missing: build it with `python tensor-ffn_b200/build.py` "
                       "(there is no CPU fallback)")
 _L = ctypes.CDLL(LIB_PATH)
 _vp, _i, _f, _cp = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_char_p
-_pp = ctypes.POINTER(ctypes.c_void_p)
+_pp, _i64 = ctypes.POINTER(ctypes.c_void_p), ctypes.c_int64
 _SIGS = {
     "tffn_last_error": (_cp, []),
     "tffn_version": (_i, []),
@@ -110,6 +117,15 @@ _SIGS = {
     "tffn_attention_cut": (_i, [_i, _i, _i, _i, _i, _i, _vp, ctypes.c_int64, _vp]),
     "tffn_prompt_attention_waits": (_i, [_vp, _i, _i, _i, _i]),
     "tffn_latent_attention_cut": (_i, [_i, _i, _i, _i, _i, _i, ctypes.c_int64, _vp]),
+    "tffn_norm_forward": (_i, [_i, _i, _i, _vp, _vp, _vp, _i64, _i, _f, _vp, _vp, _vp, _vp]),
+    "tffn_norm_backward_workspace": (_i64, [_i64, _i]),
+    "tffn_norm_backward": (_i, [_i, _i, _i] + [_vp] * 6 + [_i64, _i] + [_vp] * 4 + [_i64, _vp]),
+    "tffn_attention_forward": (_i, [_i, ctypes.POINTER(AttentionShape)] + [_vp] * 8),
+    "tffn_attention_backward_workspace": (_i64, [ctypes.POINTER(AttentionShape)]),
+    "tffn_attention_backward": (_i, [_i, ctypes.POINTER(AttentionShape)] + [_vp] * 12 + [_i64, _vp]),
+    "tffn_token_logprobs": (_i, [_i, _i, _vp, _i64, _vp, _i64, _i, _vp, _vp]),
+    "tffn_policy_loss": (_i, [_i, _i, _vp, _i64] + [_vp] * 5 + [_i64, _i, _f, _f, _f] + [_vp] * 6),
+    "tffn_train_status": (_i, [_i]),
     "tffn_op_wait_selftest": (_i, [_i]),
     "tffn_op_tp_wait_selftest": (_i, [_i, _i]),
 }
@@ -478,6 +494,68 @@ class Session:
 
     def stream(self) -> int:
         return int(_L.tffn_session_stream(self._h) or 0)
+
+
+# Training operators: every *_ptr is a device address, stream a cudaStream_t as an integer; the calls enqueue and return.
+DTYPES = {"bfloat16": 0, "float32": 1}
+NORM_KINDS = {"rms": 0, "layer": 1}
+
+
+def _code(table: dict, name: str) -> int:
+    if name not in table:
+        raise TffnError(-1, "%r is none of %s" % (name, ", ".join(sorted(table))))
+    return table[name]
+
+
+def norm_forward(kind: str, dtype: str, x_ptr, weight_ptr, bias_ptr, rows: int, width: int, eps: float, y_ptr, mean_ptr, rstd_ptr, stream: int = 0,
+                 device: int = 0):
+    """rows of an RMS ("rms") or layer ("layer") norm, and their statistics (fp32; bias and mean None for "rms")"""
+    _check(_L.tffn_norm_forward(device, _code(NORM_KINDS, kind), _code(DTYPES, dtype), x_ptr, weight_ptr, bias_ptr, rows, width, eps, y_ptr, mean_ptr,
+                                rstd_ptr, stream))
+
+
+def norm_backward_workspace(rows: int, width: int) -> int:
+    return _check(_L.tffn_norm_backward_workspace(rows, width))
+
+
+def norm_backward(kind: str, dtype: str, dy_ptr, x_ptr, weight_ptr, mean_ptr, rstd_ptr, skip_ptr, rows: int, width: int, dx_ptr, dweight_ptr, dbias_ptr,
+                  workspace_ptr, workspace_bytes: int, stream: int = 0, device: int = 0):
+    """dx (+ skip), and the fp32 sums dweight and dbias over the rows"""
+    _check(_L.tffn_norm_backward(device, _code(NORM_KINDS, kind), _code(DTYPES, dtype), dy_ptr, x_ptr, weight_ptr, mean_ptr, rstd_ptr, skip_ptr, rows, width,
+                                 dx_ptr, dweight_ptr, dbias_ptr, workspace_ptr, workspace_bytes, stream))
+
+
+def attention_forward(shape: AttentionShape, cu_q_ptr, cu_k_ptr, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, stream: int = 0, device: int = 0):
+    """attention of packed sequences; lse (fp32 [heads][rows_q]) is what the backward call needs"""
+    _check(_L.tffn_attention_forward(device, shape, cu_q_ptr, cu_k_ptr, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, stream))
+
+
+def attention_backward_workspace(shape: AttentionShape) -> int:
+    return _check(_L.tffn_attention_backward_workspace(shape))
+
+
+def attention_backward(shape: AttentionShape, cu_q_ptr, cu_k_ptr, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, d_out_ptr, dq_ptr, dk_ptr, dv_ptr,
+                       workspace_ptr, workspace_bytes: int, stream: int = 0, device: int = 0):
+    _check(_L.tffn_attention_backward(device, shape, cu_q_ptr, cu_k_ptr, q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr, d_out_ptr, dq_ptr, dk_ptr, dv_ptr,
+                                      workspace_ptr, workspace_bytes, stream))
+
+
+def token_logprobs(dtype: str, logits_ptr, targets_ptr, rows: int, vocab: int, logprob_ptr, row_stride: int = 0, stream: int = 0, device: int = 0):
+    """fp32 log-probability of one token (int32) per row of logits"""
+    _check(_L.tffn_token_logprobs(device, _code(DTYPES, dtype), logits_ptr, row_stride, targets_ptr, rows, vocab, logprob_ptr, stream))
+
+
+def policy_loss(dtype: str, logits_ptr, targets_ptr, old_logprob_ptr, ref_logprob_ptr, advantage_ptr, weight_ptr, rows: int, vocab: int, clip_low: float,
+                clip_high: float, kl_coef: float, loss_ptr, row_loss_ptr, logprob_ptr, kl_ptr, d_logits_ptr, row_stride: int = 0, stream: int = 0,
+                device: int = 0):
+    """clipped policy loss with a KL term, and its gradient to the logits"""
+    _check(_L.tffn_policy_loss(device, _code(DTYPES, dtype), logits_ptr, row_stride, targets_ptr, old_logprob_ptr, ref_logprob_ptr, advantage_ptr,
+                               weight_ptr, rows, vocab, clip_low, clip_high, kl_coef, loss_ptr, row_loss_ptr, logprob_ptr, kl_ptr, d_logits_ptr, stream))
+
+
+def train_status(device: int = 0) -> int:
+    """what the bounded waits of the training operators have reported (0: nothing); waits for the device"""
+    return _check(_L.tffn_train_status(device))
 
 
 def attention_cut(n_seqs: int, heads: int, kv_heads: int, head_dim: int, max_ctx: int, num_sms: int, resident, scratch_floats: int = 8 << 20):
