@@ -479,7 +479,7 @@ AttnCall attn_call(const tffn_attention* a) {
     need(std::isfinite(a->scale) && a->scale > 0.f, "the attention scale must be positive");
     need(a->chunk >= 0 && (a->chunk == 0 || a->causal), "chunks need a causal mask");
     if (a->head_dim % 8 || a->head_dim > 128) throw Error(kErrUnsupported, "attention heads must be a multiple of 8 wide, at most 128");
-    if (a->heads > 65535 || a->rows_q > INT32_MAX || a->rows_k > INT32_MAX) throw Error(kErrUnsupported, "more than 65535 heads or 2^31 rows");
+    if (a->heads > 65535 || a->rows_q > INT32_MAX - 4096 || a->rows_k > INT32_MAX - 4096) throw Error(kErrUnsupported, "more than 65535 heads or 2^31 rows");
     const int64_t q = (int64_t)a->heads * a->head_dim, k = (int64_t)a->kv_heads * a->head_dim;
     need(a->q_stride >= q && a->out_stride >= q && a->k_stride >= k && a->v_stride >= k, "an attention row stride is shorter than its row");
     need(a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0 && a->out_stride % 8 == 0, "attention row strides must be multiples of 8 elements");
@@ -588,7 +588,7 @@ int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* c
         c.lse = lse;
         OnDevice on(device);
         c.status = status_word(device);
-        check_launch(launch_attention_train_forward(c, (cudaStream_t)stream), "attention forward");
+        check_launch(launch_attention_train_forward(c, on.num_sms, (cudaStream_t)stream), "attention forward");
     });
 }
 int64_t tffn_attention_backward_workspace(const tffn_attention* a) {
@@ -621,7 +621,7 @@ int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* 
         c.workspace = workspace;
         OnDevice on(device);
         c.status = status_word(device);
-        check_launch(launch_attention_train_backward(c, (cudaStream_t)stream), "attention backward");
+        check_launch(launch_attention_train_backward(c, on.num_sms, (cudaStream_t)stream), "attention backward");
     });
 }
 int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, int64_t rows, int vocab, float* logprob,

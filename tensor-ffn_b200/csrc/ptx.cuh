@@ -197,6 +197,43 @@ __device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
         "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
+// Four of these in a row, a_step and b_step apart: one election and no predicate arithmetic between them, a few instructions a
+// product instead of a dozen. It matters where the issuing warp shares its scheduler with busy ones.
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void umma_bf16_x4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "add.s64 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.s64 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
+        : "memory");
+}
+// the same with A in tensor memory
+template <int A_STEP, int B_STEP>
+__device__ __forceinline__ void umma_bf16_ts_x4(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync _|q, 0xffffffff;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        "add.s32 a, %1, %5;\n\tadd.s64 b, %2, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t"
+        "add.s32 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t"
+        "add.s32 a, a, %5;\n\tadd.s64 b, b, %6;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "n"(A_STEP), "n"(B_STEP)
+        : "memory");
+}
 // 32 lanes x 16 consecutive 32-bit columns -> 16 registers per thread (thread i reads lane base+i)
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(

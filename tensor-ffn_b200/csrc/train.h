@@ -85,7 +85,7 @@ struct AttnCall {
     int* status;
 };
 int64_t attention_workspace_bytes(const AttnCall& c);
-[[nodiscard]] int launch_attention_train_forward(const AttnCall& c, cudaStream_t s);
-[[nodiscard]] int launch_attention_train_backward(const AttnCall& c, cudaStream_t s);
+[[nodiscard]] int launch_attention_train_forward(const AttnCall& c, int num_sms, cudaStream_t s);
+[[nodiscard]] int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t s);
 
 }  // namespace tffn

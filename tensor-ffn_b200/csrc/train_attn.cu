@@ -1,177 +1,153 @@
-// Attention of packed training sequences on the tensor cores, forward and backward. With P = exp(scale Q K^T - lse) inside the mask and 0
-// outside, D = rowsum(dO o O):
-//   O = P V,   lse = log rowsum exp(scale Q K^T)
-//   dS = P o (dO V^T - D),   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO
-// The backward pass forms P again from lse, so nothing of the size queries x keys is ever stored.
+// Forward pass of the attention of packed training sequences on the tensor cores (inference/src/model/qwen.cu:349-412 materialises the scores):
+//   S = scale Q K^T inside the mask,   O = softmax(S) V,   lse = log of the softmax's denominators
 //
-// One shape serves all three kernels. 128 rows stand still (queries for O and dQ, keys for dK and dV) while tiles of 64 rows of the other
-// side stream past through a ring that one warp fills by TMA:
-//   forward   S = Q K^T                       | O  += P V
-//   dQ        S = Q K^T,   dP = dO V^T        | dQ += dS K
-//   dK, dV    S^T = K Q^T, dP^T = V dO^T      | dV += P^T dO,  dK += dS^T Q
-// The left products take both operands along the head; the right ones take the streamed tile a second time, read the other way round, and
-// P or dS from the tensor memory that S or dP came from, in bf16. Standing operands lie in tensor memory, where they cost no
-// shared-memory bandwidth (in shared memory for dK, dV of 128-wide heads, which leave no room there). Thread = standing row, so that a
-// row's mask is one interval of columns and its statistics need no exchange. Two groups of four warps take alternate tiles; one's exponentials run
-// under the other's products. In the forward pass each group has a maximum, a sum and an O of its own, joined at the end.
+// A persistent block of three (64 columns a head) or two (128) groups of four warps streams tiles of 64 keys and values past units of 128 queries of
+// one head (thread = query). With few units the groups take turns at the tiles of one unit, each with a maximum, a sum and an O of its own that
+// are joined at its end, so that a unit is done sooner and uneven lengths even out; with many, each group has a unit to itself, mostly
+// heads of the same queries, which share what is fetched. S = Q K^T and O += P V are tcgen05 products; one warp fills the rings by TMA, one
+// per group issues its products. S has its columns to itself and P others, so the next S is formed as soon as a group has S in registers, and
+// a group's exponentials follow each other without waiting for the tensor cores. The next unit's queries and scores are on their way while
+// results are stored. S, sums and O are fp32; P enters its product as bf16 (half a step, 2^-9 of each term, as inputs and results have). A
+// row's reference maximum moves only when it would be passed by more than 2^8, so O is rarely rescaled.
 //
-// P and dS enter their products as bf16: half a step, 2^-9 of each term, the rounding that inputs and results have as well; S, dP, sums,
-// statistics and O, dQ, dK, dV are fp32 until they are stored.
-//
-// dQ and dK, dV are two kernels, each with its own S and dP: 7 products of a tile instead of 5, but every output row has one block that
-// adds it up in one order, so the gradients are the same bits on every run, without atomics on dQ.
-#include "launch.h"
-#include "ptx.cuh"
-#include "train.h"
+// What bounds it: 64 columns a head: the exponentials (8 192 a tile at 16 a cycle), a quarter of which therefore run as polynomials on the FMA
+// pipe; 128: the products (640 cycles a tile).
+#include "train_attn.cuh"
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace tffn {
 
 namespace {
 
-constexpr int kStand = 128, kTile = 64, kWarpsOfGroup = 4, kThreads = 320;
-constexpr float kLog2e = 1.4426950408889634f;
-enum Kind { FWD = 0, DQ = 1, DKV = 2 };
+constexpr int kTile = 64;
+#ifndef SHARE
+#define SHARE 12
+#endif
+constexpr int kShareUnits = SHARE;
 
-template <int HD, int KIND>
-struct Cfg {
-    static constexpr int BLOCKS = HD / 64;                   // column blocks of 64 (128 swizzled bytes)
-    static constexpr int BLOCK = kTile * 128, TILE = BLOCKS * BLOCK, STAGE = 2 * TILE;
-    static constexpr bool A_SHARED = KIND == DKV && HD == 128;
-    static constexpr int A_BLOCK = kStand * 128, A_TILE = A_SHARED ? BLOCKS * A_BLOCK : 0;
-    static constexpr int STAGES = 4;
-    static constexpr int RING = 2 * A_TILE, AFTER = RING + STAGES * STAGE;
-    static constexpr int BARS = AFTER, ROWS = BARS + 256;    // ROWS: lse and D of streamed queries, or the groups' statistics
-    static constexpr int SMEM = ROWS + 2 * 2 * kTile * 8;
-    // tensor memory columns
-    static constexpr int A0 = 0, A1 = HD / 2;
-    static constexpr int S = A_SHARED ? 0 : KIND == FWD ? HD / 2 : HD;
-    static constexpr int S_STEP = KIND == FWD ? kTile : 2 * kTile;         // S, and dP behind it
-    static constexpr int P = S + 2 * kTile;                                // forward only (32 columns a group); else P and dS lie where S and dP were
-    static constexpr int ACC = KIND == FWD ? P + kTile : S + 4 * kTile;    // O of each group; dQ; dK, dV
-    static constexpr int COLS = ACC + (KIND == DQ ? HD : 2 * HD);
-    static_assert(COLS <= 512 && SMEM <= 227 * 1024, "");
+// up to NG units of one kv head of a sequence, or one unit that the groups share, and the tiles of keys that they see
+template <int NG>
+struct Units {
+    int q_first, k_first, q_len, k_len, kvh;
+    int first, tiles;        // of all; tiles = -1: no more work
+    int n;
+    int a_first[NG], a_rows[NG], head[NG];
+    int t_lo[NG], t_hi[NG];  // tiles that a unit sees
 };
 
-struct Dev {
-    CUtensorMap tm[2];   // streamed operands: K, V or Q, dO; boxes of 64 rows x 64 columns of one head
-    CUtensorMap tmA[2];  // standing K, V where they lie in shared memory; boxes of 128 rows
-    const bf16 *a0, *a1; // standing rows: Q, dO or K, V
-    int64_t a0_stride, a1_stride;
-    const int *cu_q, *cu_k;
-    int64_t rows_q, rows_k;
-    int max_q, max_k, n_seqs, heads, kv_heads, hd, causal, chunk;
-    int parts;           // of the query heads of a kv head (dK, dV)
-    float scale, scale_log2;
-    float* lse;          // [heads][rows_q]
-    const float* d;      // [heads][rows_q]
-    bf16 *out0, *out1;   // O; dQ; dK, dV
-    int64_t out0_stride, out1_stride;
-    float* partial;      // parts > 1: dK, dV as fp32 [2][parts][rows_k][kv_heads][hd]
-    int* status;
-};
-
-struct Span {
-    int64_t first;
-    int len;
-};
-// rows of sequence i, whatever the offsets say inside the buffer and not longer than promised
-__device__ __forceinline__ Span span_of(const int* cu, int i, int64_t rows, int most) {
-    const int64_t b = min(max((int64_t)cu[i], (int64_t)0), rows), e = min(max((int64_t)cu[i + 1], b), rows);
-    return {b, (int)min(e - b, (int64_t)most)};
+// the units of one step of a block's walk
+template <int NG>
+__device__ __forceinline__ void units_of(const AttnDev& p, const AttnUnit& u, Units<NG>& w) {
+    w.q_first = u.q.first;
+    w.k_first = u.k.first;
+    w.q_len = u.q.len;
+    w.k_len = u.k.len;
+    w.kvh = u.fast;
+    const int blocks = (u.q.len + kStand - 1) / kStand, first_unit = u.slot * p.parts;
+    w.n = min(p.parts, blocks * p.group - first_unit);
+    int lo[NG], hi[NG], last = 0;
+    w.first = INT32_MAX;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        lo[g] = hi[g] = w.a_first[g] = w.a_rows[g] = w.head[g] = 0;
+        if (g < w.n || p.parts == 1) {
+            const int unit = first_unit + (p.parts == 1 ? 0 : g), block = p.by_group.div(unit);
+            w.head[g] = u.fast * p.group + unit - block * p.group;
+            w.a_first[g] = (blocks - 1 - block) * kStand;  // late queries see most keys: first
+            w.a_rows[g] = min(kStand, u.q.len - w.a_first[g]);
+            int unused;
+            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g], lo[g], unused);
+            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g] + w.a_rows[g] - 1, unused, hi[g]);
+        }
+        if (hi[g] > lo[g]) {
+            w.first = min(w.first, lo[g]);
+            last = max(last, hi[g]);
+        }
+    }
+    w.tiles = last > 0 ? (last - w.first + kTile - 1) / kTile : 0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const bool any = hi[g] > lo[g];
+        w.t_lo[g] = any ? (lo[g] - w.first) / kTile : 0;
+        w.t_hi[g] = any ? (hi[g] - w.first + kTile - 1) / kTile : 0;
+    }
 }
 
-__device__ __forceinline__ void group_barrier(int group) { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); }
-__device__ __forceinline__ void groups_barrier() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *(const uint32_t*)&h;
-}
-
-// a standing row (or zeros) into the calling lane's tensor memory, two columns of the head per word
 template <int HD>
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const bf16* row, int hd) {
-#pragma unroll
-    for (int c = 0; c < HD; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (row && c + 8 * i < hd) v = __ldg((const uint4*)(row + c + 8 * i));
-            w[4 * i] = v.x;
-            w[4 * i + 1] = v.y;
-            w[4 * i + 2] = v.z;
-            w[4 * i + 3] = v.w;
-        }
-        tmem_st16(taddr + c / 2, w);
-    }
-    tc_wait_st();
-}
+struct Cfg {
+    static constexpr int GROUPS = HD == 64 ? 3 : 2, THREADS = (4 * GROUPS + 4) * 32;
+    static constexpr int BLOCKS = HD / 64, BLOCK = kTile * 128, TILE = BLOCKS * BLOCK;  // column blocks of 64 (128 swizzled bytes)
+    static constexpr int Q_BLOCK = kStand * 128, Q_TILE = BLOCKS * Q_BLOCK;
+    // Queries of each group, or of the unit that they share; then the stages of the ring, K and V. Groups that share a unit hold a tile each,
+    // and have more stages instead of queries of their own.
+    static constexpr int OWN_STAGES = 4, SHARED_STAGES = HD == 64 ? 8 : 4, STAGE = 2 * TILE;  // powers of two
+    static constexpr int own_bytes = GROUPS * Q_TILE + OWN_STAGES * STAGE, shared_bytes = Q_TILE + SHARED_STAGES * STAGE;
+    static constexpr int OUT = own_bytes > shared_bytes ? own_bytes : shared_bytes;     // 2 KB a warp for its results on their way out
+    static constexpr int STATS = OUT + GROUPS * 4 * 2048;
+    static constexpr int SLOTS = STATS + GROUPS * kStand * 8, BARS = SLOTS + kUnitSlots * (int)sizeof(Units<GROUPS>), SMEM = BARS + 512;
+    static_assert(BARS % 8 == 0, "");
+    // tensor memory: S of each group, P of each group, O of each group
+    static constexpr int P = GROUPS * kTile, ACC = P + GROUPS * kTile / 2;
+    static_assert(ACC + GROUPS * HD <= 512 && SMEM <= 227 * 1024, "");
+};
 
-template <int HD, int KIND>
-__global__ void __launch_bounds__(kThreads, 1) k_train_attn(const __grid_constant__ Dev p) {
-    using C = Cfg<HD, KIND>;
+template <int HD>
+__global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_constant__ AttnDev p) {
+    using C = Cfg<HD>;
+    constexpr int NG = C::GROUPS;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint64_t* const full = (uint64_t*)(smem + C::BARS);
-    uint64_t *const empty = full + C::STAGES, *const s_full = empty + C::STAGES, *const s_free = s_full + 2, *const p_full = s_free + 2, *const p_done = p_full + 2,
-                    *const a_full = p_done + 2, *const all_done = a_full + 1;
-    uint32_t* const tmem_slot = (uint32_t*)(all_done + 1);
+    constexpr int MOST = C::SHARED_STAGES;
+    const bool own = p.parts > 1;  // each group has a unit of its own
+    const int stages = own ? C::OWN_STAGES : C::SHARED_STAGES, log_stages = __popc(stages - 1), ring_at = (own ? NG : 1) * C::Q_TILE;
+    uint64_t* const k_full = (uint64_t*)(smem + C::BARS);
+    uint64_t *const k_empty = k_full + MOST, *const v_full = k_empty + MOST, *const v_empty = v_full + MOST, *const q_full = v_empty + MOST, *const q_empty = q_full + NG, *const s_full = q_empty + NG, *const s_free = s_full + NG, *const p_full = s_free + NG, *const o_full = p_full + NG,
+                    *const o_free = o_full + NG, *const u_full = o_free + NG, *const u_empty = u_full + kUnitSlots;
+    uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
+    Units<NG>* const slots = (Units<NG>*)(smem + C::SLOTS);
+    static_assert((4 * MOST + 7 * NG + 2 * kUnitSlots) * 8 + 4 <= 512 && C::OWN_STAGES <= MOST, "");
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-
-    // ---- what this block computes
-    int unit = blockIdx.x;
-    const int fast = KIND == DKV ? p.kv_heads * p.parts : p.heads;
-    const int head = unit % fast;  // query head; kv head * parts + part
-    unit /= fast;
-    const int seq = unit % p.n_seqs, slot = unit / p.n_seqs;
-    const Span sq = span_of(p.cu_q, seq, p.rows_q, p.max_q), sk = span_of(p.cu_k, seq, p.rows_k, p.max_k);
-    const int off = sk.len - sq.len;  // position of query i: i + off
-    const int stand_len = KIND == DKV ? sk.len : sq.len, stream_len = KIND == DKV ? sq.len : sk.len;
-    const int n_slots = (stand_len + kStand - 1) / kStand;
-    if (slot >= n_slots) return;
-    // the longest first: late queries see most keys, early keys are seen by most queries
-    const int a_first = (KIND == DKV ? slot : n_slots - 1 - slot) * kStand, a_rows = min(kStand, stand_len - a_first);
-    const int G = p.heads / p.kv_heads;
-    const int kvh = KIND == DKV ? head / p.parts : head / G;
-    int h0 = head, h1 = head + 1;  // query heads
-    if (KIND == DKV) {
-        const int part = head % p.parts, per = (G + p.parts - 1) / p.parts;
-        h0 = kvh * G + min(part * per, G);
-        h1 = kvh * G + min(part * per + per, G);
-    }
-    // visible streamed rows of standing row r
-    auto visible = [&](int r, int& lo, int& hi) {
-        if (KIND == DKV) {
-            lo = p.causal ? max(0, r - off) : 0;
-            hi = p.chunk > 0 ? (int)min((int64_t)sq.len, ((int64_t)(r / p.chunk) + 1) * p.chunk - off) : sq.len;
-        } else {
-            const int pos = r + off;
-            lo = p.chunk > 0 && pos > 0 ? pos / p.chunk * p.chunk : 0;
-            hi = p.causal ? pos + 1 : sk.len;
-        }
-    };
-    int first, last, unused;
-    visible(a_first, first, unused);
-    visible(a_first + a_rows - 1, unused, last);
-    const int tiles_per_head = last > first ? (last - first + kTile - 1) / kTile : 0, tiles = tiles_per_head * (h1 - h0);
-
     if (tid == 0) {
-        for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+        for (int i = 0; i < MOST; ++i) {
+            mbar_init(&k_full[i], 1);
+            mbar_init(&k_empty[i], own ? NG : 1);
+            mbar_init(&v_full[i], 1);
+            mbar_init(&v_empty[i], own ? NG : 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NG; ++i) {
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], own ? 1 : NG);
             mbar_init(&s_full[i], 1);
             mbar_init(&s_free[i], 128);
             mbar_init(&p_full[i], 128);
-            mbar_init(&p_done[i], 1);
+            mbar_init(&o_full[i], 1);
+            mbar_init(&o_free[i], 128);
         }
-        mbar_init(a_full, C::A_SHARED ? 1 : 256);
-        mbar_init(all_done, 1);
+        for (int i = 0; i < kUnitSlots; ++i) {
+            mbar_init(&u_full[i], 1);
+            mbar_init(&u_empty[i], 2 * NG + 4 * NG);  // both walks of each product warp, each softmax warp
+        }
         fence_mbar_init();
     }
-    if (warp == 9) {
+    // The first warp works out the units. Its first one does not need the barriers.
+    int cursor = blockIdx.x;
+    Units<NG> w;
+    auto next_units = [&]() {
+        AttnUnit u;
+        w.tiles = -1;
+        if (next_unit<false>(p, cursor, u, [&](int len) { return p.by_parts.div((len + kStand - 1) / kStand * p.group + p.parts - 1); })) units_of<NG>(p, u, w);
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            prefetch_tmap(&p.tm[0]);
+            prefetch_tmap(&p.tm[1]);
+            prefetch_tmap(&p.tmA[0]);
+        }
+        __syncwarp();
+        next_units();
+    }
+    if (warp == 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
@@ -179,372 +155,363 @@ __global__ void __launch_bounds__(kThreads, 1) k_train_attn(const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    if (KIND != FWD) pdl_wait();
-
-    if (warp == 8) {
-        if (lane == 0) {
-            prefetch_tmap(&p.tm[0]);
-            prefetch_tmap(&p.tm[1]);
-        }
+    // a reader's copy of the index-th units of the block
+    auto take = [&](int index, Units<NG>& to) {
+        const int slot = index % kUnitSlots;
+        const bool there = __all_sync(0xffffffffu, mbar_wait(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
+        to = slots[slot];
+        if (!there) to.tiles = -1;
         __syncwarp();
-        const uint32_t ring = smem_u32(smem + C::RING), bar = smem_u32(full);
-        auto load = [&](const CUtensorMap* tm, uint32_t dst, int n_heads, int h, int64_t row, uint32_t b, int block) {
-#pragma unroll
-            for (int i = 0; i < C::BLOCKS; ++i)
-                if (n_heads > 1)
-                    tma_load_3d_elect(dst + i * block, tm, i * 64, h, (int)row, b);
-                else
-                    tma_load_2d_elect(dst + i * block, tm, i * 64, (int)row, b);
-        };
-        if (C::A_SHARED && tiles > 0) {
-            const uint32_t a = smem_u32(smem), ab = smem_u32(a_full);
-            mbar_arrive_expect_tx_elect(ab, 2 * C::A_TILE);
-            load(&p.tmA[0], a, p.kv_heads, kvh, sk.first + a_first, ab, C::A_BLOCK);
-            load(&p.tmA[1], a + C::A_TILE, p.kv_heads, kvh, sk.first + a_first, ab, C::A_BLOCK);
-        }
+        if (lane == 0) mbar_arrive(&u_empty[slot]);
+    };
+
+    if (warp == 0) {
+        // ---- units, and by TMA their queries, then keys and values tile by tile
+        const uint32_t base = smem_u32(smem);
+        auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
         bool ok = true;
-        int h = h0, t = 0;
-        for (int j = 0; j < tiles && ok; ++j) {
-            const int st = j % C::STAGES;
-            if (j >= C::STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (uint32_t)(j / C::STAGES - 1) & 1u, p.status, DEV_ERR_EMPTY_WAIT));
+        int st = 0, begun[NG] = {0};
+        uint32_t round = 0;
+        for (int index = 0; ok; ++index) {
+            const int slot = index % kUnitSlots;
+            if (index >= kUnitSlots) ok = wait(&u_empty[slot], (uint32_t)(index / kUnitSlots - 1) & 1u);
             if (!ok) break;
-            const uint32_t b = bar + st * 8, dst = ring + st * C::STAGE;
-            mbar_arrive_expect_tx_elect(b, C::STAGE);
-            const int64_t row = (KIND == DKV ? sq.first : sk.first) + first + t * kTile;
-            const int n_heads = KIND == DKV ? p.heads : p.kv_heads, hh = KIND == DKV ? h : kvh;
-            load(&p.tm[0], dst, n_heads, hh, row, b, C::BLOCK);
-            load(&p.tm[1], dst + C::TILE, n_heads, hh, row, b, C::BLOCK);
-            if (++t == tiles_per_head) {
-                t = 0;
-                ++h;
+            if (lane == 0) {
+                slots[slot] = w;
+                mbar_arrive(&u_full[slot]);
             }
-        }
-    } else if (warp == 9) {
-        constexpr uint32_t idesc_s = umma_idesc_bf16(kStand, kTile), idesc_acc = umma_idesc_bf16(kStand, HD) | (1u << 16);  // streamed tile: its K extent in rows
-        const uint32_t ring = smem_u32(smem + C::RING);
-        const uint64_t a_d = umma_desc_k128(smem_u32(smem)), k_d = umma_desc_k128(ring), n_d = umma_desc_n128(ring, C::BLOCK);
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
-        // S or dP of a tile: standing operand `which` times streamed operand `which`
-        auto product = [&](uint32_t d, int which, int st) {
-            const uint64_t b = k_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4);
+            __syncwarp();
+            if (w.tiles < 0) break;
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i) {
-                const uint64_t bi = b + (i >> 2) * (C::BLOCK >> 4) + 2 * (i & 3);
-                if constexpr (C::A_SHARED)
-                    umma_bf16_elect(d, a_d + (uint64_t)(uint32_t)((which * C::A_TILE + (i >> 2) * C::A_BLOCK) >> 4) + 2 * (i & 3), bi, idesc_s, i > 0);
-                else
-                    umma_bf16_ts(d, tmem + (which ? C::A1 : C::A0) + i * 8, bi, idesc_s, i > 0);
-            }
-        };
-        auto accumulate = [&](uint32_t d, uint32_t a, int which, int st, bool more) {
-            const uint64_t b = n_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4);
-#pragma unroll
-            for (int i = 0; i < kTile / 16; ++i) umma_bf16_ts(d, a + i * 8, b + i * 128, idesc_acc, more || i > 0);
-        };
-        auto scores = [&](int j) {
-            const int st = j % C::STAGES;
-            if (!wait(&full[st], (uint32_t)(j / C::STAGES) & 1u, DEV_ERR_FULL_WAIT)) return false;
-            const int valid = stream_len - first - j % tiles_per_head * kTile;
-            if (valid < kTile) {
-                // rows behind the sequence weigh zero, but what lies there may not be finite
-                for (int i = lane; i < (kTile - valid) * 8 * 2 * C::BLOCKS; i += 32) {
-                    const int c = i & 7, b = (i >> 3) % (2 * C::BLOCKS), r = valid + (i >> 3) / (2 * C::BLOCKS);
-                    *(uint4*)(smem + C::RING + st * C::STAGE + b * C::BLOCK + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+            for (int g = 0; g < NG; ++g)
+                if (ok && w.t_hi[g] > w.t_lo[g] && (own || g == 0)) {
+                    if (begun[g] > 0) ok = wait(&q_empty[g], (uint32_t)(begun[g] - 1) & 1u);
+                    if (ok) {
+                        mbar_arrive_expect_tx_elect(smem_u32(&q_full[g]), C::Q_TILE);
+                        load_head<C::BLOCKS>(&p.tmA[0], base + g * C::Q_TILE, C::Q_BLOCK, p.heads, w.head[g], w.q_first + w.a_first[g], smem_u32(&q_full[g]));
+                    }
+                    ++begun[g];
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
+            for (int t = 0; t < w.tiles && ok; ++t) {
+                const int row = w.k_first + w.first + t * kTile;
+                if (round > 0) ok = wait(&k_empty[st], (round - 1) & 1u);
+                if (!ok) break;
+                mbar_arrive_expect_tx_elect(smem_u32(&k_full[st]), C::TILE);
+                load_head<C::BLOCKS>(&p.tm[0], base + ring_at + st * C::STAGE, C::BLOCK, p.kv_heads, w.kvh, row, smem_u32(&k_full[st]));
+                if (round > 0) ok = wait(&v_empty[st], (round - 1) & 1u);
+                if (!ok) break;
+                mbar_arrive_expect_tx_elect(smem_u32(&v_full[st]), C::TILE);
+                load_head<C::BLOCKS>(&p.tm[1], base + ring_at + st * C::STAGE + C::TILE, C::BLOCK, p.kv_heads, w.kvh, row, smem_u32(&v_full[st]));
+                if (++st == stages) {
+                    st = 0;
+                    ++round;
+                }
             }
-            tc_fence_after();
-            const uint32_t d = tmem + C::S + (j & 1) * C::S_STEP;
-            product(d, 0, st);
-            if (KIND != FWD) product(d + kTile, 1, st);
-            umma_commit_elect(&s_full[j & 1]);
+            if (ok) next_units();
+        }
+    } else if (warp <= NG) {
+        // ---- products of one group: S runs up to two tiles ahead of P V
+        const int g = warp - 1;
+        constexpr uint32_t idesc_s = umma_idesc_bf16(kStand, kTile), idesc_o = umma_idesc_bf16(kStand, HD) | (1u << 16);  // V: its K extent in rows
+        const uint32_t base = smem_u32(smem);
+        const uint64_t q_d = umma_desc_k128(base + (own ? g * C::Q_TILE : 0)), k_d = umma_desc_k128(base + ring_at), v_d = umma_desc_n128(base + ring_at + C::TILE, C::BLOCK);
+        const int qb = own ? g : 0;
+        const uint32_t s_at = tmem + g * kTile, p_at = tmem + C::P + g * (kTile / 2), acc = tmem + C::ACC + g * HD;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
+        // Two walks over the same tiles, that of S and behind it that of P V. A group that has a unit of its own takes every tile of the block,
+        // since a stage of the ring is free when all groups are past it, and passes on those that it does not see.
+        struct Walk {
+            int tiles = 0, first = 0, k_len = 0, t = 0, t_lo = 0, t_hi = 0;
+            int base = 0, index = 0, slot = 0;  // tiles and number of the units with tiles before; units taken
+            uint32_t done = 0, units = 0;       // this group's tiles; units whose queries, whose O it has begun
+            bool more = true;
+            __device__ __forceinline__ bool has() const { return more && t < tiles; }
+        } ahead, now;
+        const int step = own ? 1 : NG;
+        auto enter = [&](Walk& k) {
+            k.base += k.tiles;
+            k.index += k.tiles > 0;
+            take(k.slot++, w);
+            k.more = w.tiles >= 0;
+            k.tiles = max(w.tiles, 0);
+            k.first = w.first;
+            k.k_len = w.k_len;
+            k.t = k.t_lo = own ? 0 : g;
+            k.t_hi = k.tiles;
+            if (own)
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    if (i == g) {
+                        k.t_lo = w.t_lo[i];
+                        k.t_hi = w.t_hi[i];
+                    }
+        };
+        // Both walks to their next tiles. Units go to the first walk first, and it stays close enough to the second for the slots; while the
+        // second still has products to issue, which the warp that hands out units may be waiting for, the first takes only what is there.
+        auto settle = [&]() {
+            for (;;) {
+                if (!ahead.has() && ahead.more && ahead.slot < now.slot + kUnitSlots &&
+                    (!now.has() || __all_sync(0xffffffffu, mbar_try_wait(&u_full[ahead.slot % kUnitSlots], (uint32_t)(ahead.slot / kUnitSlots) & 1u)))) {
+                    enter(ahead);
+                    if (!own && ahead.tiles > 0 && g >= ahead.tiles) ++ahead.units;  // fewer tiles than groups: the first lets go of the queries in this one's place
+                } else if (!now.has() && now.more && now.slot < ahead.slot) {
+                    enter(now);
+                } else {
+                    break;
+                }
+            }
+        };
+        bool ok = true;
+        auto scores = [&]() {
+            const int n = ahead.base + ahead.t, st = n & (stages - 1), t = ahead.t;
+            if (!wait(&k_full[st], (uint32_t)(n >> log_stages) & 1u, DEV_ERR_FULL_WAIT)) return false;
+            if (t >= ahead.t_lo && t < ahead.t_hi) {
+                if (t == ahead.t_lo && !wait(&q_full[qb], ahead.units & 1u, DEV_ERR_FULL_WAIT)) return false;
+                if (ahead.done > 0 && !wait(&s_free[g], (ahead.done - 1) & 1u, DEV_ERR_ACC_WAIT)) return false;
+                ++ahead.done;
+                tc_fence_after();
+                const uint64_t b = k_d + (uint64_t)(uint32_t)((st * C::STAGE) >> 4);
+#pragma unroll
+                for (int i = 0; i < C::BLOCKS; ++i) umma_bf16_x4<2, 2>(s_at, q_d + i * (C::Q_BLOCK >> 4), b + i * (C::BLOCK >> 4), idesc_s, i > 0);
+                umma_commit_elect(&s_full[g]);
+                umma_commit_elect(&k_empty[st]);
+                if (t + step >= ahead.t_hi) {
+                    umma_commit_elect(&q_empty[qb]);
+                    if (!own && g == 0 && lane == 0)
+                        for (int i = ahead.t_hi; i < NG; ++i) mbar_arrive(&q_empty[qb]);
+                    ++ahead.units;
+                }
+            } else if (lane == 0) {
+                mbar_arrive(&k_empty[st]);
+            }
+            ahead.t += step;
             return true;
         };
-        bool ok = tiles > 0 && wait(a_full, 0, DEV_ERR_FULL_WAIT);
-        tc_fence_after();
-        if (ok) ok = scores(0);
-        if (ok && tiles > 1) ok = scores(1);
-        for (int j = 0; j < tiles && ok; ++j) {
-            const int st = j % C::STAGES, b = j & 1;
-            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-            if (KIND == FWD && j + 2 < tiles) {  // S of this tile is in registers: the next one of its group takes its place
-                ok = wait(&s_free[b], ph, DEV_ERR_ACC_WAIT) && scores(j + 2);
-                if (!ok) break;
+        // S two tiles ahead, but not of a tile that can only be fetched when the one that P V is at has left the ring, nor of a unit whose
+        // queries can only be fetched when the groups have joined the results of the unit that P V is at
+        for (int lead = 0; ok; --lead) {
+            settle();
+            if (!now.has()) break;
+            const int n = now.base + now.t, st = n & (stages - 1), t = now.t;
+            while (ok && lead < 2 && ahead.has() && ahead.base + ahead.t - n < stages && ahead.index <= now.index + 1) {
+                ok = scores();
+                ++lead;
+                settle();
             }
-            ok = wait(&p_full[b], ph, DEV_ERR_ACC_WAIT);
             if (!ok) break;
-            tc_fence_after();
-            if constexpr (KIND == FWD) {
-                accumulate(tmem + C::ACC + b * HD, tmem + C::P + b * (kTile / 2), 1, st, j > 1);
-                umma_commit_elect(&p_done[b]);
-            } else if constexpr (KIND == DQ) {
-                accumulate(tmem + C::ACC, tmem + C::S + b * C::S_STEP, 0, st, j > 0);
-            } else {
-                accumulate(tmem + C::ACC + HD, tmem + C::S + b * C::S_STEP, 1, st, j > 0);      // dV
-                accumulate(tmem + C::ACC, tmem + C::S + b * C::S_STEP + kTile, 0, st, j > 0);   // dK
+            ok = wait(&v_full[st], (uint32_t)(n >> log_stages) & 1u, DEV_ERR_FULL_WAIT);
+            if (!ok) break;
+            if (t >= now.t_lo && t < now.t_hi) {
+                const int valid = now.k_len - now.first - t * kTile;
+                if (valid < kTile) zero_rows(smem + ring_at + st * C::STAGE + C::TILE, C::BLOCK, C::BLOCKS, valid, kTile);
+                ok = wait(&p_full[g], now.done & 1u, DEV_ERR_ACC_WAIT);
+                ++now.done;
+                if (ok && t == now.t_lo) {
+                    if (now.units > 0) ok = wait(&o_free[g], (now.units - 1) & 1u, DEV_ERR_ACC_WAIT);
+                    ++now.units;
+                }
+                if (!ok) break;
+                tc_fence_after();
+                umma_bf16_ts_x4<8, 128>(acc, p_at, v_d + (uint64_t)(uint32_t)((st * C::STAGE) >> 4), idesc_o, t > now.t_lo);
+                umma_commit_elect(&o_full[g]);
+                umma_commit_elect(&v_empty[st]);
+            } else if (lane == 0) {
+                mbar_arrive(&v_empty[st]);
             }
-            umma_commit_elect(&empty[st]);
-            if (KIND != FWD && j + 2 < tiles) ok = scores(j + 2);  // behind the products that read this buffer
+            now.t += step;
         }
-        if (ok && tiles > 0) umma_commit_elect(all_done);
-    } else {
-        const int group = warp / kWarpsOfGroup, r = tid % kStand;
-        const uint32_t lanes = (uint32_t)((warp % kWarpsOfGroup) * 32) << 16;
-        const bool live = r < a_rows;
-        const int row = a_first + r;
-        const int64_t grow = (KIND == DKV ? sk.first : sq.first) + row;  // row of the buffers
-        const int a_head = KIND == DKV ? kvh : head;
+    } else if (warp >= 4) {
+        // ---- softmax
+        const int g = (warp >> 2) - 1, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, buf = tmem + lanes + g * kTile, p_at = tmem + lanes + C::P + g * (kTile / 2), acc = tmem + lanes + C::ACC + g * HD;
+        uint8_t* const mine = smem + C::OUT + (warp - 4) * 2048;
+        float2* const stats = (float2*)(smem + C::STATS);
         bool ok = true;
-        if (!C::A_SHARED && tiles > 0) {
-            if (group == 0 || KIND != FWD) {
-                const bf16* src = group == 0 ? p.a0 + grow * p.a0_stride : p.a1 + grow * p.a1_stride;
-                row_to_tmem<HD>(tmem + lanes + (group == 0 ? C::A0 : C::A1), live ? src + (int64_t)a_head * p.hd : nullptr, p.hd);
-            }
-            tc_fence_before();
-            mbar_arrive(a_full);
-        }
-        int lo = 0, hi = 0;
-        if (live) visible(row, lo, hi);
-        float2* const stats = (float2*)(smem + C::ROWS);
-        float m = -INFINITY, sum = 0.f, lse2 = 0.f, dd = 0.f;
-        if (KIND == DQ && live) {
-            const float l = p.lse[(int64_t)head * p.rows_q + grow];
-            lse2 = l == -INFINITY ? 0.f : l * kLog2e;
-            dd = p.d[(int64_t)head * p.rows_q + grow];
-        }
-        // lse (first half of the group) and D (second half) of a streamed query
-        auto fetch = [&](int j) {
-            if (j >= tiles) return 0.f;
-            const int col = first + j % tiles_per_head * kTile + (r & 63), h = h0 + j / tiles_per_head;
-            if (col >= sq.len) return 0.f;
-            const float v = __ldg((r < 64 ? p.lse : p.d) + (int64_t)h * p.rows_q + sq.first + col);
-            return r < 64 ? (v == -INFINITY ? 0.f : v * kLog2e) : v;
-        };
-        float ahead = KIND == DKV ? fetch(group) : 0.f;
-        // A wait that ran out lets the warp go on without waiting, since the others of its group wait for it at their barrier.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, DEV_ERR_ACC_WAIT));
-        };
-        for (int j = group; j < tiles; j += 2) {
-            const int b = group;
-            const uint32_t ph = (uint32_t)(j >> 1) & 1u;
-            const uint32_t buf = tmem + lanes + C::S + b * C::S_STEP;
-            const int base = first + j % tiles_per_head * kTile;
-            const int c_lo = lo - base, c_hi = hi - base;  // visible columns
-            const bool whole = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= kTile);
-            float2* const q_stats = stats + (b * 2 + (int)ph) * kTile;
-            if (KIND == DKV) {
-                ((float*)(q_stats + (r & 63)))[r < 64 ? 0 : 1] = ahead;
-                ahead = fetch(j + 2);
-                group_barrier(group);
-            }
-            wait(&s_full[b], ph);
             tc_fence_after();
-            if constexpr (KIND == FWD) {
+        };
+        uint32_t turns = 0;  // tiles so far
+        for (int index = 0;; ++index) {
+            take(index, w);
+            if (w.tiles < 0) break;
+            int a_first = 0, a_rows = 0, head = 0, t_lo = 0, t_hi = 0;
+#pragma unroll
+            for (int i = 0; i < NG; ++i)
+                if (i == g) {
+                    a_first = w.a_first[i];
+                    a_rows = w.a_rows[i];
+                    head = w.head[i];
+                    t_lo = w.t_lo[i];
+                    t_hi = w.t_hi[i];
+                }
+            if (own && g >= w.n) continue;
+            const int begin = own ? t_lo : g, step = own ? 1 : NG;
+            const bool live = r < a_rows;
+            const int64_t grow = w.q_first + a_first + r;  // row of the buffers
+            int lo = 0, hi = 0;
+            if (live) attn_visible<false>(p, w.q_len, w.k_len, a_first + r, lo, hi);
+            float m = -INFINITY, sum = 0.f;
+            for (int t = begin; t < t_hi; t += step, ++turns) {
+                const int c_lo = lo - w.first - t * kTile, c_hi = hi - w.first - t * kTile;  // visible columns
+                const bool whole = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= kTile);
+                wait(&s_full[g], turns & 1u);
                 uint32_t s[4][16];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tmem_ld16(buf + k * 16, s[k]);
                 tc_wait_ld();
                 tc_fence_before();
-                mbar_arrive(&s_free[b]);
+                mbar_arrive(&s_free[g]);
                 if (!whole)
 #pragma unroll
                     for (int i = 0; i < kTile; ++i)
                         if (i < c_lo || i >= c_hi) s[i >> 4][i & 15] = 0xff800000u;
-                float top = -INFINITY;
+                auto at = [&](int i) { return __uint_as_float(s[i >> 4][i & 15]); };
+                float tops[2] = {fmaxf(at(0), at(1)), fmaxf(at(2), at(3))};
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) top = fmaxf(top, __uint_as_float(s[i >> 4][i & 15]));
-                top *= p.scale_log2;  // positive scale: the maximum stays the maximum
+                for (int i = 4; i < kTile; i += 2) tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], at(i), at(i + 1));
+                const float top = fmaxf(tops[0], tops[1]) * p.scale_log2;  // positive scale: the maximum stays the maximum
                 float corr = 1.f;
                 bool moved = false;
-                if (top > m + 8.f || m == -INFINITY) {  // the reference moves only when it would be passed by more than 2^8
+                if (top > m + 8.f || m == -INFINITY) {
                     corr = m == -INFINITY ? 0.f : exp2_fast(m - top);
                     moved = m != -INFINITY;
                     m = top;
                 }
                 const float ref = m == -INFINITY ? 0.f : m;  // nothing visible yet: every weight is zero
                 sum *= corr;
-                uint32_t w[2][16];
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                const F2 scale2 = f2(p.scale_log2, p.scale_log2), ref2 = f2(-ref, -ref);
+                uint32_t v[2][16];
+                F2 part[2] = {0ull, 0ull};
+                // every fourth pair by polynomial where the whole tile is visible (it has no zero)
+                auto weights = [&](auto poly) {
 #pragma unroll
-                for (int i = 0; i < kTile; i += 2) {
-                    const float x = exp2_fast(fmaf(__uint_as_float(s[i >> 4][i & 15]), p.scale_log2, -ref));
-                    const float y = exp2_fast(fmaf(__uint_as_float(s[i >> 4][(i & 15) + 1]), p.scale_log2, -ref));
-                    part[i >> 1 & 3] += x + y;
-                    w[i >> 5][(i & 31) >> 1] = pack2(x, y);
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                if (j > 1) {  // the product that read the last P, and wrote O
-                    wait(&p_done[b], ((uint32_t)(j >> 1) - 1u) & 1u);
-                    tc_fence_after();
-                }
+                    for (int i = 0; i < kTile; i += 2) {
+                        const F2 x = fma2(f2(at(i), at(i + 1)), scale2, ref2);
+                        float a, b;
+                        if (poly.value && i % 8 == 6) {
+                            split2(exp2_poly(x), a, b);
+                        } else {
+                            split2(x, a, b);
+                            a = exp2_fast(a);
+                            b = exp2_fast(b);
+                        }
+                        part[i >> 1 & 1] = add2(part[i >> 1 & 1], f2(a, b));
+                        v[i >> 5][(i & 31) >> 1] = pack2(a, b);
+                    }
+                };
+                if (whole)
+                    weights(std::true_type());
+                else
+                    weights(std::false_type());
+                float parts[4];
+                split2(part[0], parts[0], parts[1]);
+                split2(part[1], parts[2], parts[3]);
+                sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
+                if (t > begin) wait(&o_full[g], (turns - 1) & 1u);  // the product that read the last P, and wrote O
                 if (__any_sync(0xffffffffu, moved)) {
-                    const uint32_t o_at = tmem + lanes + C::ACC + b * HD;
 #pragma unroll 1
                     for (int k = 0; k < HD / 16; ++k) {
                         uint32_t o[16];
-                        tmem_ld16(o_at + k * 16, o);
+                        tmem_ld16(acc + k * 16, o);
                         tc_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                        tmem_st16(o_at + k * 16, o);
+                        tmem_st16(acc + k * 16, o);
                     }
                 }
-                tmem_st16(tmem + lanes + C::P + b * (kTile / 2), w[0]);
-                tmem_st16(tmem + lanes + C::P + b * (kTile / 2) + 16, w[1]);
+                tmem_st16(p_at, v[0]);
+                tmem_st16(p_at + 16, v[1]);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[g]);
+            }
+            // ---- results of the unit
+            const bool any = t_hi > begin;
+            if (any) wait(&o_full[g], (turns - 1) & 1u);
+            const int warp_row = (warp & 3) * 32;
+            char* const dst = (char*)(p.out0 + (int64_t)(w.q_first + a_first + warp_row) * p.out0_stride + (int64_t)head * p.hd);
+            float weight[NG];  // of each group's O
+            if (own) {
+                weight[0] = sum > 0.f ? 1.f / sum : 0.f;
             } else {
+                stats[g * kStand + r] = make_float2(m, sum);
+                tc_fence_before();
+                named_barrier(1, NG * 128);
+                tc_fence_after();
+                float top = -INFINITY;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t s[2][16], dp[2][16], w[16], v[16];
+                for (int i = 0; i < NG; ++i) top = fmaxf(top, stats[i * kStand + r].x);
+                sum = 0.f;
+                m = top;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        tmem_ld16(buf + half * 32 + k * 16, s[k]);
-                        tmem_ld16(buf + kTile + half * 32 + k * 16, dp[k]);
-                    }
+                for (int i = 0; i < NG; ++i) {
+                    const float2 x = stats[i * kStand + r];
+                    weight[i] = x.x == -INFINITY ? 0.f : exp2_fast(x.x - top);
+                    sum = fmaf(x.y, weight[i], sum);
+                }
+                const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) weight[i] *= inv;
+            }
+            if (live && p.lse && (own || g == 0)) p.lse[(int64_t)head * p.rows_q + grow] = sum > 0.f ? (m + log2f(sum)) / kLog2e : -INFINITY;
+            // a group's own O, or its share of the columns of the joined one
+#pragma unroll 1
+            for (int c = own ? 0 : 32 * g; c < HD; c += own ? 32 : 32 * NG) {
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = 0.f;
+                auto add = [&](uint32_t from, float f) {
+                    uint32_t x[2][16];
+                    tmem_ld16(from + c, x[0]);
+                    tmem_ld16(from + c + 16, x[1]);
                     tc_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        float pr[2], ds[2];
-                        float4 st4;
-                        if constexpr (KIND == DKV) st4 = *(const float4*)(q_stats + half * 32 + i);
+                    for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(x[i >> 4][i & 15]), f, o[i]);
+                };
+                if (own) {
+                    if (any) add(acc, weight[0]);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int c = half * 32 + i + e;
-                            const float l = KIND == DKV ? (e ? st4.z : st4.x) : lse2, dr = KIND == DKV ? (e ? st4.w : st4.y) : dd;
-                            float x = exp2_fast(fmaf(__uint_as_float(s[i >> 4][(i & 15) + e]), p.scale_log2, -l));
-                            if (!whole && (c < c_lo || c >= c_hi)) x = 0.f;
-                            pr[e] = x;
-                            ds[e] = x * (__uint_as_float(dp[i >> 4][(i & 15) + e]) - dr);
-                        }
-                        w[i >> 1] = pack2(pr[0], pr[1]);
-                        v[i >> 1] = pack2(ds[0], ds[1]);
-                    }
-                    if constexpr (KIND == DKV) {
-                        tmem_st16(buf + half * 16, w);
-                        tmem_st16(buf + kTile + half * 16, v);
-                    } else {
-                        tmem_st16(buf + half * 16, v);
-                    }
+                    for (int i = 0; i < NG; ++i)
+                        if (t_hi > i) add(tmem + lanes + C::ACC + i * HD, weight[i]);
                 }
+                uint4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = make_uint4(pack2(o[8 * i], o[8 * i + 1]), pack2(o[8 * i + 2], o[8 * i + 3]), pack2(o[8 * i + 4], o[8 * i + 5]), pack2(o[8 * i + 6], o[8 * i + 7]));
+                store_rows(mine, v, dst + c * 2, p.out0_stride * 2, a_rows - warp_row, (p.hd - c) / 8);
             }
-            tc_wait_st();
             tc_fence_before();
-            mbar_arrive(&p_full[b]);
-        }
-        // ---- results
-        if (tiles > 0) wait(all_done, 0);
-        tc_fence_after();
-        float w0 = tiles > 0 ? 1.f : 0.f, w1 = 0.f;  // weights of the accumulators
-        if constexpr (KIND == FWD) {
-            stats[group * kStand + r] = make_float2(m, sum);
-            groups_barrier();
-            const float2 x = stats[r], y = stats[kStand + r];
-            const float top = fmaxf(x.x, y.x);
-            const float e0 = x.x == -INFINITY ? 0.f : exp2_fast(x.x - top), e1 = y.x == -INFINITY ? 0.f : exp2_fast(y.x - top);
-            const float total = fmaf(x.y, e0, y.y * e1);
-            w0 = total > 0.f ? e0 / total : 0.f;
-            w1 = total > 0.f ? e1 / total : 0.f;
-            if (group == 0 && live && p.lse) p.lse[(int64_t)head * p.rows_q + grow] = total > 0.f ? (top + log2f(total)) / kLog2e : -INFINITY;
-        } else {
-            w0 *= KIND == DQ || group == 0 ? p.scale : 1.f;
-        }
-        // FWD, DQ: a group stores half of the columns; DKV: dK, dV
-        constexpr int WIDTH = KIND == DKV ? HD : HD / 2;
-        const int col0 = KIND == DKV ? 0 : group * WIDTH;
-        const uint32_t acc = tmem + lanes + C::ACC + (KIND == DKV ? group * HD : col0);
-        bf16* const dst = KIND == DKV && group == 1 ? p.out1 + grow * p.out1_stride : p.out0 + grow * p.out0_stride;
-        float* const part = KIND == DKV && p.partial
-                                ? p.partial + ((((int64_t)group * p.parts + head % p.parts) * p.rows_k + grow) * p.kv_heads + kvh) * p.hd
-                                : nullptr;
-#pragma unroll 1
-        for (int k = 0; k < WIDTH / 16; ++k) {
-            float v[16];
-            uint32_t o[16], o2[16];
-            if (tiles > 0) tmem_ld16(acc + k * 16, o);
-            if (KIND == FWD && tiles > 1) tmem_ld16(acc + HD + k * 16, o2);
-            tc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                v[i] = tiles > 0 ? __uint_as_float(o[i]) * w0 : 0.f;
-                if (KIND == FWD && tiles > 1) v[i] = fmaf(__uint_as_float(o2[i]), w1, v[i]);
-            }
-            const int c = col0 + k * 16;
-#pragma unroll
-            for (int i = 0; i < 16; i += 8)
-                if (live && c + i < p.hd) {
-                    if (KIND == DKV && part) {
-                        *(float4*)(part + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                        *(float4*)(part + c + i + 4) = make_float4(v[i + 4], v[i + 5], v[i + 6], v[i + 7]);
-                    } else {
-                        *(uint4*)(dst + (int64_t)a_head * p.hd + c + i) =
-                            make_uint4(pack2(v[i], v[i + 1]), pack2(v[i + 2], v[i + 3]), pack2(v[i + 4], v[i + 5]), pack2(v[i + 6], v[i + 7]));
-                    }
-                }
-            __syncwarp();
+            if (!own) named_barrier(1, NG * 128);  // every group has read every O, and the statistics
+            if (any) mbar_arrive(&o_free[g]);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) tmem_dealloc(tmem, 512);
+    if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// D[h][row] = sum of dO o O over the head: L = HD / 8 lanes a row, neighbouring rows in neighbouring lanes
-template <int L>
-__global__ void __launch_bounds__(256) k_attn_dot(const bf16* __restrict__ d_out, const bf16* __restrict__ out, int64_t stride, const int* cu_q, int n_seqs, int64_t rows, int heads,
-                                                  int hd, float* __restrict__ d) {
-    pdl_launch_dependents();
-    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const int h = blockIdx.y, c = threadIdx.x % L * 8;
-    const bool live = row < rows && row >= cu_q[0] && row < cu_q[n_seqs];
-    float a = 0.f;
-    if (live && c < hd) {
-        const uint4 x = __ldg((const uint4*)(d_out + row * stride + (int64_t)h * hd + c)), y = __ldg((const uint4*)(out + row * stride + (int64_t)h * hd + c));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a = fmaf(bf16_lo(xs[i]), bf16_lo(ys[i]), a);
-            a = fmaf(bf16_hi(xs[i]), bf16_hi(ys[i]), a);
-        }
-    }
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-    if (live && c == 0) d[(int64_t)h * rows + row] = a;
-}
-
-// dK and dV from the parts of the query heads, added in their order
-__global__ void __launch_bounds__(256) k_attn_join(const float* __restrict__ partial, int parts, const int* cu_k, int n_seqs, int64_t rows, int kv_heads, int hd, bf16* dk,
-                                                   int64_t dk_stride, bf16* dv, int64_t dv_stride) {
-    pdl_wait();
-    const int per_row = kv_heads * hd / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
-    if (row >= rows || row < cu_k[0] || row >= cu_k[n_seqs]) return;
-    const int c = (int)(i % per_row) * 4;
-    const int64_t plane = rows * kv_heads * hd;
-    const float* src = partial + (int64_t)blockIdx.y * parts * plane + row * kv_heads * hd + c;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < parts; ++q) {
-        const float4 v = __ldg((const float4*)(src + q * plane));
-        a.x += v.x;
-        a.y += v.y;
-        a.z += v.z;
-        a.w += v.w;
-    }
-    bf16* dst = blockIdx.y ? dv + row * dv_stride : dk + row * dk_stride;
-    *(uint2*)(dst + c) = make_uint2(pack2(a.x, a.y), pack2(a.z, a.w));
-}
-
-template <int HD, int KIND>
-int run(const Dev& p, int64_t blocks, cudaStream_t s, bool pdl) {
-    using C = Cfg<HD, KIND>;
-    const cudaError_t e = allow_shared<k_train_attn<HD, KIND>>(C::SMEM);
+template <int HD>
+int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
+    using C = Cfg<HD>;
+    const int G = c.heads / c.kv_heads;
+    const int64_t blocks = (c.max_q + kStand - 1) / kStand, all = blocks * c.n_seqs * c.heads;
+    p.parts = all <= kShareUnits * num_sms ? 1 : C::GROUPS;
+    const int64_t units = (blocks * G + p.parts - 1) / p.parts * c.n_seqs * c.kv_heads;
+    if (units >= 1 << 30 || blocks * G >= 1 << 30) return (int)cudaErrorInvalidValue;
+    p.units = (int)units;
+    p.by_fast = FastDiv::of(c.kv_heads);
+    p.by_parts = FastDiv::of(p.parts);
+    const cudaError_t e = allow_shared<k_attn_fwd<HD>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    if (blocks > INT32_MAX) return (int)cudaErrorInvalidValue;
-    return (int)launch_k(k_train_attn<HD, KIND>, dim3((unsigned)blocks), dim3(kThreads), (size_t)C::SMEM, s, pdl, p);
+    return (int)launch_k(k_attn_fwd<HD>, dim3((unsigned)(p.units < num_sms ? p.units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, false, p);
 }
 
-Dev common(const AttnCall& c) {
-    Dev p;
+}  // namespace
+
+AttnDev attn_dev(const AttnCall& c) {
+    AttnDev p;
     memset(&p, 0, sizeof p);
     p.cu_q = c.cu_q;
     p.cu_k = c.cu_k;
@@ -555,6 +522,11 @@ Dev common(const AttnCall& c) {
     p.n_seqs = c.n_seqs;
     p.heads = c.heads;
     p.kv_heads = c.kv_heads;
+    p.group = c.heads / c.kv_heads;
+    p.by_group = FastDiv::of(p.group);
+    p.by_seqs = FastDiv::of(c.n_seqs);
+    p.by_chunk = FastDiv::of(c.chunk > 0 ? c.chunk : 1);
+    p.by_fast = p.by_parts = FastDiv::of(1);
     p.hd = c.hd;
     p.causal = c.causal;
     p.chunk = c.chunk;
@@ -570,97 +542,17 @@ bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int
     return make_tmap_2d(nullptr, tm, x, (uint64_t)rows, (uint64_t)hd, (uint64_t)stride, (uint32_t)box, (uint32_t)heads, (uint32_t)hd);
 }
 
-int64_t blocks_for(const AttnCall& c, int most, int fast) { return (int64_t)((most + kStand - 1) / kStand) * c.n_seqs * fast; }
-
-// Blocks of dK, dV by query heads: one block adds all heads of its kv head up where that gives each of the 148 SMs two blocks to even out
-// unequal lengths; else the heads are dealt to as many blocks as that takes, and their sums are joined through the workspace.
-int parts_of(const AttnCall& c) {
-    const int G = c.heads / c.kv_heads;
-    const int64_t blocks = blocks_for(c, c.max_k, c.kv_heads);
-    int parts = 1;
-    while (parts < G && blocks * parts < 2 * 148) ++parts;
-    const int per = (G + parts - 1) / parts;
-    return (G + per - 1) / per;
-}
-
-}  // namespace
-
-int64_t attention_workspace_bytes(const AttnCall& c) {
-    const int64_t d = ((int64_t)c.heads * c.rows_q * 4 + 255) / 256 * 256;
-    const int parts = parts_of(c);
-    return d + (parts > 1 ? 2 * parts * c.rows_k * c.kv_heads * c.hd * 4 : 0);
-}
-
-int launch_attention_train_forward(const AttnCall& c, cudaStream_t s) {
+int launch_attention_train_forward(const AttnCall& c, int num_sms, cudaStream_t s) {
     if (c.n_seqs == 0 || c.max_q == 0 || c.rows_q == 0) return 0;
-    Dev p = common(c);
-    // no keys at all: any valid map, none of its rows is read
-    if (!map_heads(&p.tm[0], c.rows_k ? c.k : c.q, c.rows_k ? c.rows_k : c.rows_q, c.rows_k ? c.k_stride : c.q_stride, c.kv_heads, c.hd, kTile)) return -1000;
-    if (!map_heads(&p.tm[1], c.rows_k ? c.v : c.q, c.rows_k ? c.rows_k : c.rows_q, c.rows_k ? c.v_stride : c.q_stride, c.kv_heads, c.hd, kTile)) return -1000;
-    p.a0 = c.q;
-    p.a0_stride = c.q_stride;
+    AttnDev p = attn_dev(c);
+    if (!map_heads(&p.tmA[0], c.q, c.rows_q, c.q_stride, c.heads, c.hd, kStand)) return -1000;
+    p.tm[0] = p.tm[1] = p.tmA[0];  // no keys at all: any valid map, none of its rows is read
+    if (c.rows_k > 0 && c.max_k > 0 &&
+        (!map_heads(&p.tm[0], c.k, c.rows_k, c.k_stride, c.kv_heads, c.hd, kTile) || !map_heads(&p.tm[1], c.v, c.rows_k, c.v_stride, c.kv_heads, c.hd, kTile)))
+        return -1000;
     p.out0 = c.out;
     p.out0_stride = c.out_stride;
-    const int64_t blocks = blocks_for(c, c.max_q, c.heads);
-    return c.hd <= 64 ? run<64, FWD>(p, blocks, s, false) : run<128, FWD>(p, blocks, s, false);
-}
-
-int launch_attention_train_backward(const AttnCall& c, cudaStream_t s) {
-    const bool queries = c.max_q > 0 && c.rows_q > 0, keys = c.max_k > 0 && c.rows_k > 0;
-    if (c.n_seqs == 0 || (!queries && !keys)) return 0;
-    float* const d = (float*)c.workspace;
-    int rc = 0;
-    if (queries) {
-        const int lanes = c.hd <= 64 ? 8 : 16;
-        const dim3 grid((unsigned)((c.rows_q + 256 / lanes - 1) / (256 / lanes)), (unsigned)c.heads);
-        rc = lanes == 8 ? (int)launch_k(k_attn_dot<8>, grid, dim3(256), 0, s, false, c.d_out, c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d)
-                        : (int)launch_k(k_attn_dot<16>, grid, dim3(256), 0, s, false, c.d_out, c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d);
-        if (rc) return rc;
-    }
-    if (keys) {
-        Dev p = common(c);
-        const bf16 *q = queries ? c.q : c.k, *g = queries ? c.d_out : c.k;  // no queries: any valid map, none of its rows is read
-        const int64_t rows = queries ? c.rows_q : c.rows_k;
-        if (!map_heads(&p.tm[0], q, rows, queries ? c.q_stride : c.k_stride, queries ? c.heads : c.kv_heads, c.hd, kTile)) return -1000;
-        if (!map_heads(&p.tm[1], g, rows, queries ? c.out_stride : c.k_stride, queries ? c.heads : c.kv_heads, c.hd, kTile)) return -1000;
-        if (!map_heads(&p.tmA[0], c.k, c.rows_k, c.k_stride, c.kv_heads, c.hd, kStand)) return -1000;
-        if (!map_heads(&p.tmA[1], c.v, c.rows_k, c.v_stride, c.kv_heads, c.hd, kStand)) return -1000;
-        p.a0 = c.k;
-        p.a0_stride = c.k_stride;
-        p.a1 = c.v;
-        p.a1_stride = c.v_stride;
-        p.d = d;
-        p.parts = parts_of(c);
-        p.partial = p.parts > 1 ? (float*)((char*)c.workspace + ((int64_t)c.heads * c.rows_q * 4 + 255) / 256 * 256) : nullptr;
-        p.out0 = c.dk;
-        p.out0_stride = c.k_stride;
-        p.out1 = c.dv;
-        p.out1_stride = c.v_stride;
-        const int64_t blocks = blocks_for(c, c.max_k, c.kv_heads * p.parts);
-        rc = c.hd <= 64 ? run<64, DKV>(p, blocks, s, false) : run<128, DKV>(p, blocks, s, false);
-        if (rc) return rc;
-        if (p.partial) {
-            const int64_t vecs = c.rows_k * c.kv_heads * c.hd / 4;
-            rc = (int)launch_k(k_attn_join, dim3((unsigned)((vecs + 255) / 256), 2), dim3(256), 0, s, false, (const float*)p.partial, p.parts, c.cu_k, c.n_seqs, c.rows_k, c.kv_heads,
-                               c.hd, c.dk, c.k_stride, c.dv, c.v_stride);
-            if (rc) return rc;
-        }
-    }
-    if (queries) {
-        Dev p = common(c);
-        if (!map_heads(&p.tm[0], keys ? c.k : c.q, keys ? c.rows_k : c.rows_q, keys ? c.k_stride : c.q_stride, c.kv_heads, c.hd, kTile)) return -1000;
-        if (!map_heads(&p.tm[1], keys ? c.v : c.q, keys ? c.rows_k : c.rows_q, keys ? c.v_stride : c.q_stride, c.kv_heads, c.hd, kTile)) return -1000;
-        p.a0 = c.q;
-        p.a0_stride = c.q_stride;
-        p.a1 = c.d_out;
-        p.a1_stride = c.out_stride;
-        p.d = d;
-        p.out0 = c.dq;
-        p.out0_stride = c.q_stride;
-        const int64_t blocks = blocks_for(c, c.max_q, c.heads);
-        rc = c.hd <= 64 ? run<64, DQ>(p, blocks, s, false) : run<128, DQ>(p, blocks, s, false);
-    }
-    return rc;
+    return c.hd <= 64 ? run<64>(p, c, num_sms, s) : run<128>(p, c, num_sms, s);
 }
 
 }  // namespace tffn

@@ -1,0 +1,211 @@
+// What the forward and backward kernels of training attention (train_attn.cu, train_attn_bwd.cu) share: the call as the device sees it,
+// which rows a block computes and which it can see, and small helpers.
+#pragma once
+#include "launch.h"
+#include "ptx.cuh"
+#include "train.h"
+
+namespace tffn {
+
+constexpr int kStand = 128;  // rows that stand still: queries for O and dQ, keys for dK and dV
+constexpr float kLog2e = 1.4426950408889634f;
+
+// n / d for 0 <= n < 2^31 by a multiplication: with 2^(l - 1) < d <= 2^l, m = ceil(2^(31 + l) / d) < 2^32
+struct FastDiv {
+    uint32_t d, m, s;
+    __host__ static FastDiv of(int64_t d) {
+        FastDiv f;
+        int l = 0;
+        while ((int64_t)1 << l < d) ++l;
+        f.d = (uint32_t)d;
+        f.s = 31 + l;
+        f.m = (uint32_t)((((uint64_t)1 << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d);
+        return f;
+    }
+    __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> s); }
+};
+
+struct AttnDev {
+    CUtensorMap tm[2];   // streamed operands: K, V or Q, dO; boxes of rows x 64 columns of one head
+    CUtensorMap tmA[2];  // standing operands, boxes of 128 rows
+    const int *cu_q, *cu_k;
+    int64_t rows_q, rows_k;
+    int max_q, max_k, n_seqs, heads, kv_heads, group, hd, causal, chunk;  // group: query heads of a kv head
+    FastDiv by_fast, by_seqs, by_group, by_parts, by_chunk;               // by_fast: units of a block of standing rows of a sequence
+    int units;           // blocks' worth of work, empty ones included
+    int parts;           // units that a block takes at once (forward); parts of the query heads of a kv head (dK, dV)
+    float scale, scale_log2;
+    float* lse;          // [heads][rows_q]
+    float* d;            // [heads][rows_q]
+    bf16 *out0, *out1;   // O; dQ; dK, dV
+    int64_t out0_stride, out1_stride;
+    float* partial;      // parts > 1: dK, dV as fp32 [2][parts][rows_k][kv_heads][hd]
+    int* status;
+};
+
+// rows of a sequence, whatever the offsets say inside the buffer and not longer than promised
+struct AttnSpan {
+    int first, len;
+};
+__device__ __forceinline__ AttnSpan attn_span(int begin, int end, int64_t rows, int most) {
+    const int b = min(max(begin, 0), (int)rows), e = min(max(end, b), (int)rows);
+    return {b, min(e - b, most)};
+}
+
+// visible streamed rows [lo, hi) of standing row r: of a query, or of a key (DKV)
+template <bool DKV>
+__device__ __forceinline__ void attn_visible(const AttnDev& p, int q_len, int k_len, int r, int& lo, int& hi) {
+    const int off = k_len - q_len;  // position of query i: i + off
+    if (DKV) {
+        lo = p.causal ? max(0, r - off) : 0;
+        hi = p.chunk > 0 ? (int)min((int64_t)q_len, ((int64_t)p.by_chunk.div(r) + 1) * p.chunk - off) : q_len;
+    } else {
+        const int pos = r + off;
+        lo = p.chunk > 0 && pos > 0 ? p.by_chunk.div(pos) * p.chunk : 0;
+        hi = p.causal ? pos + 1 : k_len;
+    }
+}
+
+// A block walks over the units cursor, cursor + grid, ... A unit is (fast, sequence, slot): heads fastest, so that blocks that stream the same
+// rows run together, then the sequences, then the blocks of standing rows. `slots_of` says how many slots a sequence has.
+struct AttnUnit {
+    int fast, slot;
+    AttnSpan q, k;
+};
+// The next unit at or after `cursor` whose sequence reaches that far, for a whole warp: 32 candidates at a time, each lane with the offsets of
+// its own, which the found one hands to the others.
+template <bool DKV, typename F>
+__device__ __forceinline__ bool next_unit(const AttnDev& p, int& cursor, AttnUnit& u, F&& slots_of) {
+    const int step = gridDim.x;
+    for (;;) {
+        if (cursor >= p.units) return false;
+        const int64_t mine = (int64_t)cursor + (int64_t)(threadIdx.x & 31) * step;
+        bool there = false;
+        int fast = 0, slot = 0;
+        AttnSpan q = {0, 0}, k = {0, 0};
+        if (mine < p.units) {
+            const int rest = p.by_fast.div((int)mine);
+            fast = (int)mine - rest * (int)p.by_fast.d;
+            slot = p.by_seqs.div(rest);
+            const int seq = rest - slot * p.n_seqs;
+            const int q0 = p.cu_q[seq], q1 = p.cu_q[seq + 1], k0 = p.cu_k[seq], k1 = p.cu_k[seq + 1];
+            q = attn_span(q0, q1, p.rows_q, p.max_q);
+            k = attn_span(k0, k1, p.rows_k, p.max_k);
+            there = slot < slots_of(DKV ? k.len : q.len);
+        }
+        const unsigned found = __ballot_sync(0xffffffffu, there);
+        if (found) {
+            const int from = __ffs(found) - 1;
+            u.fast = __shfl_sync(0xffffffffu, fast, from);
+            u.slot = __shfl_sync(0xffffffffu, slot, from);
+            u.q.first = __shfl_sync(0xffffffffu, q.first, from);
+            u.q.len = __shfl_sync(0xffffffffu, q.len, from);
+            u.k.first = __shfl_sync(0xffffffffu, k.first, from);
+            u.k.len = __shfl_sync(0xffffffffu, k.len, from);
+            cursor = (int)min((int64_t)cursor + (int64_t)(from + 1) * step, (int64_t)p.units);
+            return true;
+        }
+        if ((int64_t)cursor + 32ll * step >= p.units) return false;
+        cursor += 32 * step;
+    }
+}
+
+// What one warp has worked out of a unit reaches the others through a few slots of shared memory, each with a barrier for the warps that read it
+// and one for the warp that fills it. A slot is free again when every reader has copied it.
+constexpr int kUnitSlots = 4;
+
+// boxes of 64 columns of `rows` rows of one head, block bytes apart in shared memory
+template <int BLOCKS>
+__device__ __forceinline__ void load_head(const CUtensorMap* tm, uint32_t dst, int block, int n_heads, int head, int row, uint32_t bar) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+        if (n_heads > 1)
+            tma_load_3d_elect(dst + i * block, tm, i * 64, head, row, bar);
+        else
+            tma_load_2d_elect(dst + i * block, tm, i * 64, row, bar);
+}
+// Zeros in rows [valid, rows) of `blocks` blocks of 128-byte rows, by a whole warp: rows behind a sequence weigh zero, but what lies there
+// may not be finite. For operands that only the calling warp's products read.
+__device__ __forceinline__ void zero_rows(uint8_t* at, int block, int blocks, int valid, int rows) {
+    for (int i = threadIdx.x & 31; i < (rows - valid) * 8 * blocks; i += 32) {
+        const int c = i & 7, b = (i >> 3) % blocks, r = valid + (i >> 3) / blocks;
+        *(uint4*)(at + b * block + r * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// ---- two fp32 values in one register pair
+typedef unsigned long long F2;
+__device__ __forceinline__ F2 f2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void split2(F2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two values below 127 on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by a polynomial of degree 4 fitted for the least largest
+// relative error (2.7e-6, Remez exchange), n added to its exponent. Values below -126 give 2^-126.
+__device__ __forceinline__ F2 exp2_poly(F2 x) {
+    float a, b;
+    split2(x, a, b);
+    x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const float big = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, which is then the low bits
+    const F2 t = add2(x, f2(big, big)), f = fma2(add2(t, f2(-big, -big)), f2(-1.f, -1.f), x);
+    F2 y = f2(0.009570102207362652f, 0.009570102207362652f);
+    y = fma2(y, f, f2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, f2(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, f2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, f2(0.9999992847442627f, 0.9999992847442627f));
+    float ya, yb, ta, tb;
+    split2(y, ya, yb);
+    split2(t, ta, tb);
+    return f2(__int_as_float(__float_as_int(ya) + (__float_as_int(ta) << 23)), __int_as_float(__float_as_int(yb) + (__float_as_int(tb) << 23)));
+}
+
+// 64 bytes of each of a warp's 32 rows (lane = row) to rows `row_bytes` apart: through 2 KB of shared memory, so that four lanes write a row's
+// 64 bytes and no sector is written in halves. `rows` rows and `pieces` of 16 bytes are written.
+__device__ __forceinline__ void store_rows(uint8_t* mine, const uint4 (&v)[4], char* to, int64_t row_bytes, int rows, int pieces) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(uint4*)(mine + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4)) = v[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), c = lane & 3;
+        const uint4 x = *(const uint4*)(mine + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+        if (r < rows && c < pieces) *(uint4*)(to + r * row_bytes + c * 16) = x;
+    }
+    __syncwarp();
+}
+
+__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *(const uint32_t*)&h;
+}
+
+// host side (train_attn.cu)
+AttnDev attn_dev(const AttnCall& c);
+bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box);
+
+}  // namespace tffn
