@@ -4,11 +4,11 @@
 // A persistent block of three (64 columns a head) or two (128) groups of four warps streams tiles of 64 keys and values past units of 128 queries of
 // one head (thread = query). With few units the groups take turns at the tiles of one unit, each with a maximum, a sum and an O of its own that
 // are joined at its end, so that a unit is done sooner and uneven lengths even out; with many, each group has a unit to itself, mostly
-// heads of the same queries, which share what is fetched. S = Q K^T and O += P V are tcgen05 products; one warp fills the rings by TMA, one
-// per group issues its products. S has its columns to itself and P others, so the next S is formed as soon as a group has S in registers, and
-// a group's exponentials follow each other without waiting for the tensor cores. The next unit's queries and scores are on their way while
-// results are stored. S, sums and O are fp32; P enters its product as bf16 (half a step, 2^-9 of each term, as inputs and results have). A
-// row's reference maximum moves only when it would be passed by more than 2^8, so O is rarely rescaled.
+// heads of the same queries, which share what is fetched. S = Q K^T and O += P V are tcgen05 products. One warp works out the units and fills the
+// rings by TMA, one per group issues its products. S has its columns to itself and P others, so the next S is formed as soon as a group has S
+// in registers, and a group's exponentials follow each other without waiting for the tensor cores. The next unit's queries and scores are on their
+// way while results are stored. S, sums and O are fp32; P enters its product as bf16 (half a step, 2^-9 of each term, as inputs and results
+// have). A row's reference maximum moves only when it would be passed by more than 2^8, so O is rarely rescaled.
 //
 // What bounds it: 64 columns a head: the exponentials (8 192 a tile at 16 a cycle), a quarter of which therefore run as polynomials on the FMA
 // pipe; 128: the products (640 cycles a tile).
@@ -22,19 +22,14 @@ namespace tffn {
 namespace {
 
 constexpr int kTile = 64;
-#ifndef SHARE
-#define SHARE 12
-#endif
-constexpr int kShareUnits = SHARE;
 
-// up to NG units of one kv head of a sequence, or one unit that the groups share, and the tiles of keys that they see
+// up to NG units of one kv head of a sequence, or one unit that the groups share, and the tiles of keys that any of them sees
 template <int NG>
 struct Units {
     int q_first, k_first, q_len, k_len, kvh;
-    int first, tiles;        // of all; tiles = -1: no more work
+    int first, tiles;  // tiles = -1: no more work
     int n;
     int a_first[NG], a_rows[NG], head[NG];
-    int t_lo[NG], t_hi[NG];  // tiles that a unit sees
 };
 
 // the units of one step of a block's walk
@@ -47,32 +42,26 @@ __device__ __forceinline__ void units_of(const AttnDev& p, const AttnUnit& u, Un
     w.kvh = u.fast;
     const int blocks = (u.q.len + kStand - 1) / kStand, first_unit = u.slot * p.parts;
     w.n = min(p.parts, blocks * p.group - first_unit);
-    int lo[NG], hi[NG], last = 0;
+    int last = 0;
     w.first = INT32_MAX;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        lo[g] = hi[g] = w.a_first[g] = w.a_rows[g] = w.head[g] = 0;
-        if (g < w.n || p.parts == 1) {
-            const int unit = first_unit + (p.parts == 1 ? 0 : g), block = p.by_group.div(unit);
+        w.a_first[g] = w.a_rows[g] = w.head[g] = 0;
+        if (g < w.n) {
+            const int unit = first_unit + g, block = p.by_group.div(unit);
             w.head[g] = u.fast * p.group + unit - block * p.group;
             w.a_first[g] = (blocks - 1 - block) * kStand;  // late queries see most keys: first
             w.a_rows[g] = min(kStand, u.q.len - w.a_first[g]);
-            int unused;
-            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g], lo[g], unused);
-            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g] + w.a_rows[g] - 1, unused, hi[g]);
-        }
-        if (hi[g] > lo[g]) {
-            w.first = min(w.first, lo[g]);
-            last = max(last, hi[g]);
+            int lo, hi, unused;
+            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g], lo, unused);
+            attn_visible<false>(p, u.q.len, u.k.len, w.a_first[g] + w.a_rows[g] - 1, unused, hi);
+            if (hi > lo) {
+                w.first = min(w.first, lo);
+                last = max(last, hi);
+            }
         }
     }
     w.tiles = last > 0 ? (last - w.first + kTile - 1) / kTile : 0;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const bool any = hi[g] > lo[g];
-        w.t_lo[g] = any ? (lo[g] - w.first) / kTile : 0;
-        w.t_hi[g] = any ? (hi[g] - w.first + kTile - 1) / kTile : 0;
-    }
 }
 
 template <int HD>
@@ -80,13 +69,13 @@ struct Cfg {
     static constexpr int GROUPS = HD == 64 ? 3 : 2, THREADS = (4 * GROUPS + 4) * 32;
     static constexpr int BLOCKS = HD / 64, BLOCK = kTile * 128, TILE = BLOCKS * BLOCK;  // column blocks of 64 (128 swizzled bytes)
     static constexpr int Q_BLOCK = kStand * 128, Q_TILE = BLOCKS * Q_BLOCK;
-    // Queries of each group, or of the unit that they share; then the stages of the ring, K and V. Groups that share a unit hold a tile each,
-    // and have more stages instead of queries of their own.
-    static constexpr int OWN_STAGES = 4, SHARED_STAGES = HD == 64 ? 8 : 4, STAGE = 2 * TILE;  // powers of two
-    static constexpr int own_bytes = GROUPS * Q_TILE + OWN_STAGES * STAGE, shared_bytes = Q_TILE + SHARED_STAGES * STAGE;
+    // Queries of each group, or of the unit that they share; then the stages of the ring, K and V. Groups that share a unit have a part of the ring
+    // each: a barrier's parity tells only the next phase from the last one, so whoever waits for a stage has to be the one that saw its last phase.
+    static constexpr int OWN_STAGES = 4, PART = HD == 64 ? 3 : 2, STAGE = 2 * TILE;
+    static constexpr int own_bytes = GROUPS * Q_TILE + OWN_STAGES * STAGE, shared_bytes = Q_TILE + GROUPS * PART * STAGE;
     static constexpr int OUT = own_bytes > shared_bytes ? own_bytes : shared_bytes;     // 2 KB a warp for its results on their way out
     static constexpr int STATS = OUT + GROUPS * 4 * 2048;
-    static constexpr int SLOTS = STATS + GROUPS * kStand * 8, BARS = SLOTS + kUnitSlots * (int)sizeof(Units<GROUPS>), SMEM = BARS + 512;
+    static constexpr int SLOTS = STATS + GROUPS * kStand * 8, BARS = SLOTS + kUnitSlots * (int)sizeof(Units<GROUPS>), SMEM = BARS + 640;
     static_assert(BARS % 8 == 0, "");
     // tensor memory: S of each group, P of each group, O of each group
     static constexpr int P = GROUPS * kTile, ACC = P + GROUPS * kTile / 2;
@@ -96,17 +85,17 @@ struct Cfg {
 template <int HD>
 __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_constant__ AttnDev p) {
     using C = Cfg<HD>;
-    constexpr int NG = C::GROUPS;
+    constexpr int NG = C::GROUPS, MOST = NG * C::PART;
     extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr int MOST = C::SHARED_STAGES;
     const bool own = p.parts > 1;  // each group has a unit of its own
-    const int stages = own ? C::OWN_STAGES : C::SHARED_STAGES, log_stages = __popc(stages - 1), ring_at = (own ? NG : 1) * C::Q_TILE;
+    const int part = own ? C::OWN_STAGES : C::PART, ring_at = (own ? NG : 1) * C::Q_TILE;
     uint64_t* const k_full = (uint64_t*)(smem + C::BARS);
-    uint64_t *const k_empty = k_full + MOST, *const v_full = k_empty + MOST, *const v_empty = v_full + MOST, *const q_full = v_empty + MOST, *const q_empty = q_full + NG, *const s_full = q_empty + NG, *const s_free = s_full + NG, *const p_full = s_free + NG, *const o_full = p_full + NG,
-                    *const o_free = o_full + NG, *const u_full = o_free + NG, *const u_empty = u_full + kUnitSlots;
+    uint64_t *const k_empty = k_full + MOST, *const v_full = k_empty + MOST, *const v_empty = v_full + MOST, *const q_full = v_empty + MOST, *const q_empty = q_full + NG,
+                    *const s_full = q_empty + NG, *const s_free = s_full + NG, *const p_full = s_free + NG, *const o_full = p_full + NG, *const o_free = o_full + NG,
+                    *const u_full = o_free + NG, *const u_empty = u_full + kUnitSlots;
     uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
     Units<NG>* const slots = (Units<NG>*)(smem + C::SLOTS);
-    static_assert((4 * MOST + 7 * NG + 2 * kUnitSlots) * 8 + 4 <= 512 && C::OWN_STAGES <= MOST, "");
+    static_assert((4 * MOST + 7 * NG + 2 * kUnitSlots) * 8 + 4 <= 640 && C::OWN_STAGES <= MOST, "");
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < MOST; ++i) {
@@ -126,7 +115,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         }
         for (int i = 0; i < kUnitSlots; ++i) {
             mbar_init(&u_full[i], 1);
-            mbar_init(&u_empty[i], 2 * NG + 4 * NG);  // both walks of each product warp, each softmax warp
+            mbar_init(&u_empty[i], NG + 4 * NG);
         }
         fence_mbar_init();
     }
@@ -155,14 +144,25 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    // a reader's copy of the index-th units of the block
-    auto take = [&](int index, Units<NG>& to) {
+    // a place in a ring, or in a group's part of it
+    struct Place {
+        int stage = 0;
+        uint32_t parity = 0;
+        __device__ __forceinline__ void step(int part) {
+            if (++stage == part) {
+                stage = 0;
+                parity ^= 1u;
+            }
+        }
+    };
+    // a reader's copy of the index-th units of the block; false if there are no more
+    auto take = [&](int index) {
         const int slot = index % kUnitSlots;
         const bool there = __all_sync(0xffffffffu, mbar_wait(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
-        to = slots[slot];
-        if (!there) to.tiles = -1;
+        w = slots[slot];
         __syncwarp();
         if (lane == 0) mbar_arrive(&u_empty[slot]);
+        return there && w.tiles >= 0;
     };
 
     if (warp == 0) {
@@ -170,8 +170,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         const uint32_t base = smem_u32(smem);
         auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
         bool ok = true;
-        int st = 0, begun[NG] = {0};
-        uint32_t round = 0;
+        int begun[NG] = {0};
+        Place fill[NG];
+        uint32_t first_round = (1u << NG) - 1u;  // of each part of the ring
         for (int index = 0; ok; ++index) {
             const int slot = index % kUnitSlots;
             if (index >= kUnitSlots) ok = wait(&u_empty[slot], (uint32_t)(index / kUnitSlots - 1) & 1u);
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
             if (w.tiles < 0) break;
 #pragma unroll
             for (int g = 0; g < NG; ++g)
-                if (ok && w.t_hi[g] > w.t_lo[g] && (own || g == 0)) {
+                if (ok && w.tiles > 0 && g < w.n) {
                     if (begun[g] > 0) ok = wait(&q_empty[g], (uint32_t)(begun[g] - 1) & 1u);
                     if (ok) {
                         mbar_arrive_expect_tx_elect(smem_u32(&q_full[g]), C::Q_TILE);
@@ -193,172 +194,153 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                     ++begun[g];
                 }
             for (int t = 0; t < w.tiles && ok; ++t) {
-                const int row = w.k_first + w.first + t * kTile;
-                if (round > 0) ok = wait(&k_empty[st], (round - 1) & 1u);
+                const int row = w.k_first + w.first + t * kTile, to = own ? 0 : t % NG;
+                Place at = fill[0];
+#pragma unroll
+                for (int i = 1; i < NG; ++i)
+                    if (i == to) at = fill[i];
+                const int st = to * (own ? 0 : C::PART) + at.stage;
+                const bool fresh = first_round >> to & 1u;
+                if (!fresh) ok = wait(&k_empty[st], at.parity ^ 1u);
                 if (!ok) break;
                 mbar_arrive_expect_tx_elect(smem_u32(&k_full[st]), C::TILE);
                 load_head<C::BLOCKS>(&p.tm[0], base + ring_at + st * C::STAGE, C::BLOCK, p.kv_heads, w.kvh, row, smem_u32(&k_full[st]));
-                if (round > 0) ok = wait(&v_empty[st], (round - 1) & 1u);
+                if (!fresh) ok = wait(&v_empty[st], at.parity ^ 1u);
                 if (!ok) break;
                 mbar_arrive_expect_tx_elect(smem_u32(&v_full[st]), C::TILE);
                 load_head<C::BLOCKS>(&p.tm[1], base + ring_at + st * C::STAGE + C::TILE, C::BLOCK, p.kv_heads, w.kvh, row, smem_u32(&v_full[st]));
-                if (++st == stages) {
-                    st = 0;
-                    ++round;
-                }
+                at.step(part);
+                if (at.stage == 0) first_round &= ~(1u << to);
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+                    if (i == to) fill[i] = at;
             }
             if (ok) next_units();
         }
     } else if (warp <= NG) {
-        // ---- products of one group: S runs up to two tiles ahead of P V
-        const int g = warp - 1;
+        // ---- products of one group
+        const int g = warp - 1, qb = own ? g : 0, step = own ? 1 : NG, begin = own ? 0 : g;
         constexpr uint32_t idesc_s = umma_idesc_bf16(kStand, kTile), idesc_o = umma_idesc_bf16(kStand, HD) | (1u << 16);  // V: its K extent in rows
-        const uint32_t base = smem_u32(smem);
-        const uint64_t q_d = umma_desc_k128(base + (own ? g * C::Q_TILE : 0)), k_d = umma_desc_k128(base + ring_at), v_d = umma_desc_n128(base + ring_at + C::TILE, C::BLOCK);
-        const int qb = own ? g : 0;
-        const uint32_t s_at = tmem + g * kTile, p_at = tmem + C::P + g * (kTile / 2), acc = tmem + C::ACC + g * HD;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
-        // Two walks over the same tiles, that of S and behind it that of P V. A group that has a unit of its own takes every tile of the block,
-        // since a stage of the ring is free when all groups are past it, and passes on those that it does not see.
-        struct Walk {
-            int tiles = 0, first = 0, k_len = 0, t = 0, t_lo = 0, t_hi = 0;
-            int base = 0, index = 0, slot = 0;  // tiles and number of the units with tiles before; units taken
-            uint32_t done = 0, units = 0;       // this group's tiles; units whose queries, whose O it has begun
-            bool more = true;
-            __device__ __forceinline__ bool has() const { return more && t < tiles; }
-        } ahead, now;
-        const int step = own ? 1 : NG;
-        auto enter = [&](Walk& k) {
-            k.base += k.tiles;
-            k.index += k.tiles > 0;
-            take(k.slot++, w);
-            k.more = w.tiles >= 0;
-            k.tiles = max(w.tiles, 0);
-            k.first = w.first;
-            k.k_len = w.k_len;
-            k.t = k.t_lo = own ? 0 : g;
-            k.t_hi = k.tiles;
-            if (own)
-#pragma unroll
-                for (int i = 0; i < NG; ++i)
-                    if (i == g) {
-                        k.t_lo = w.t_lo[i];
-                        k.t_hi = w.t_hi[i];
-                    }
-        };
-        // Both walks to their next tiles. Units go to the first walk first, and it stays close enough to the second for the slots; while the
-        // second still has products to issue, which the warp that hands out units may be waiting for, the first takes only what is there.
-        auto settle = [&]() {
-            for (;;) {
-                if (!ahead.has() && ahead.more && ahead.slot < now.slot + kUnitSlots &&
-                    (!now.has() || __all_sync(0xffffffffu, mbar_try_wait(&u_full[ahead.slot % kUnitSlots], (uint32_t)(ahead.slot / kUnitSlots) & 1u)))) {
-                    enter(ahead);
-                    if (!own && ahead.tiles > 0 && g >= ahead.tiles) ++ahead.units;  // fewer tiles than groups: the first lets go of the queries in this one's place
-                } else if (!now.has() && now.more && now.slot < ahead.slot) {
-                    enter(now);
-                } else {
-                    break;
-                }
-            }
-        };
+        const uint32_t base = smem_u32(smem), s_at = tmem + g * kTile, p_at = tmem + C::P + g * (kTile / 2), o_at = tmem + C::ACC + g * HD;
+        const int ring0 = own ? 0 : g * C::PART;  // this group's part
+        uint8_t* const ring = smem + ring_at + ring0 * C::STAGE;
+        uint64_t *const kf = k_full + ring0, *const ke = k_empty + ring0, *const vf = v_full + ring0, *const ve = v_empty + ring0;
+        const uint64_t q_d = umma_desc_k128(base + qb * C::Q_TILE), k_d = umma_desc_k128(smem_u32(ring)), v_d = umma_desc_n128(smem_u32(ring) + C::TILE, C::BLOCK);
         bool ok = true;
-        auto scores = [&]() {
-            const int n = ahead.base + ahead.t, st = n & (stages - 1), t = ahead.t;
-            if (!wait(&k_full[st], (uint32_t)(n >> log_stages) & 1u, DEV_ERR_FULL_WAIT)) return false;
-            if (t >= ahead.t_lo && t < ahead.t_hi) {
-                if (t == ahead.t_lo && !wait(&q_full[qb], ahead.units & 1u, DEV_ERR_FULL_WAIT)) return false;
-                if (ahead.done > 0 && !wait(&s_free[g], (ahead.done - 1) & 1u, DEV_ERR_ACC_WAIT)) return false;
-                ++ahead.done;
-                tc_fence_after();
-                const uint64_t b = k_d + (uint64_t)(uint32_t)((st * C::STAGE) >> 4);
-#pragma unroll
-                for (int i = 0; i < C::BLOCKS; ++i) umma_bf16_x4<2, 2>(s_at, q_d + i * (C::Q_BLOCK >> 4), b + i * (C::BLOCK >> 4), idesc_s, i > 0);
-                umma_commit_elect(&s_full[g]);
-                umma_commit_elect(&k_empty[st]);
-                if (t + step >= ahead.t_hi) {
-                    umma_commit_elect(&q_empty[qb]);
-                    if (!own && g == 0 && lane == 0)
-                        for (int i = ahead.t_hi; i < NG; ++i) mbar_arrive(&q_empty[qb]);
-                    ++ahead.units;
-                }
-            } else if (lane == 0) {
-                mbar_arrive(&k_empty[st]);
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
+        // two at once: a barrier that is ready costs 90 cycles to look at
+        auto wait_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+            const bool x = mbar_try_wait(a, pa), y = mbar_try_wait(b, pb);
+            if (!__all_sync(0xffffffffu, x && y)) {
+                wait(a, pa, DEV_ERR_FULL_WAIT);
+                wait(b, pb, DEV_ERR_ACC_WAIT);
             }
-            ahead.t += step;
-            return true;
         };
-        // S two tiles ahead, but not of a tile that can only be fetched when the one that P V is at has left the ring, nor of a unit whose
-        // queries can only be fetched when the groups have joined the results of the unit that P V is at
-        for (int lead = 0; ok; --lead) {
-            settle();
-            if (!now.has()) break;
-            const int n = now.base + now.t, st = n & (stages - 1), t = now.t;
-            while (ok && lead < 2 && ahead.has() && ahead.base + ahead.t - n < stages && ahead.index <= now.index + 1) {
-                ok = scores();
-                ++lead;
-                settle();
-            }
-            if (!ok) break;
-            ok = wait(&v_full[st], (uint32_t)(n >> log_stages) & 1u, DEV_ERR_FULL_WAIT);
-            if (!ok) break;
-            if (t >= now.t_lo && t < now.t_hi) {
-                const int valid = now.k_len - now.first - t * kTile;
-                if (valid < kTile) zero_rows(smem + ring_at + st * C::STAGE + C::TILE, C::BLOCK, C::BLOCKS, valid, kTile);
-                ok = wait(&p_full[g], now.done & 1u, DEV_ERR_ACC_WAIT);
-                ++now.done;
-                if (ok && t == now.t_lo) {
-                    if (now.units > 0) ok = wait(&o_free[g], (now.units - 1) & 1u, DEV_ERR_ACC_WAIT);
-                    ++now.units;
+        auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)); };
+        Place ks, vs;
+        auto scores = [&](bool last) {
+            tc_fence_after();
+            const uint64_t b = k_d + (uint64_t)(uint32_t)((ks.stage * C::STAGE) >> 4);
+#pragma unroll
+            for (int i = 0; i < C::BLOCKS; ++i) umma_bf16_x4<2, 2>(s_at, q_d + i * (C::Q_BLOCK >> 4), b + i * (C::BLOCK >> 4), idesc_s, i > 0);
+            umma_commit_elect(&s_full[g]);
+            umma_commit_elect(&ke[ks.stage]);
+            if (last) umma_commit_elect(&q_empty[qb]);
+            ks.step(part);
+        };
+        uint32_t turns = 0, units = 0, results = 0;  // tiles of this group so far; units whose queries have come; units with a result of this group
+        bool ahead = false;                          // S of the unit's first tile has been issued
+        for (int index = 0; ok && take(index); ++index) {
+            const int tiles = w.tiles;
+            if (own && g >= w.n) {  // no unit for this group: it passes the tiles on
+                for (int t = 0; t < tiles && ok; ++t) {
+                    wait(&kf[ks.stage], ks.parity, DEV_ERR_FULL_WAIT);
+                    if (lane == 0) mbar_arrive(&ke[ks.stage]);
+                    ks.step(part);
+                    wait(&vf[vs.stage], vs.parity, DEV_ERR_FULL_WAIT);
+                    if (lane == 0) mbar_arrive(&ve[vs.stage]);
+                    vs.step(part);
                 }
+                continue;
+            }
+            const int last_valid = w.k_len - w.first;
+            if (begin < tiles && !ahead) {
+                wait(&q_full[qb], units & 1u, DEV_ERR_FULL_WAIT);
+                wait(&kf[ks.stage], ks.parity, DEV_ERR_FULL_WAIT);
+                if (ok) scores(begin + step >= tiles);
+            }
+            ahead = false;
+            if (tiles > 0 && begin >= tiles) {  // fewer tiles than groups: the shared queries are let go all the same, once they are there
+                wait(&q_full[qb], units & 1u, DEV_ERR_FULL_WAIT);
+                if (ok && lane == 0) mbar_arrive(&q_empty[qb]);
+            }
+            units += tiles > 0;
+            for (int t = begin; t < tiles && ok; t += step, ++turns) {
+                // S of the next tile, as soon as the group has this one in registers; of the next unit's first if that is there already
+                if (t + step < tiles) {
+                    wait_both(&kf[ks.stage], ks.parity, &s_free[g], turns & 1u);
+                    if (ok) scores(t + 2 * step >= tiles);
+                } else {
+                    const int after = index + 1, at = after % kUnitSlots;
+                    if (there(&u_full[at], (uint32_t)(after / kUnitSlots) & 1u)) {
+                        const int more = slots[at].tiles;
+                        if (begin < more && (!own || g < slots[at].n) && there(&q_full[qb], units & 1u) && there(&kf[ks.stage], ks.parity)) {
+                            wait(&s_free[g], turns & 1u, DEV_ERR_ACC_WAIT);
+                            if (ok) scores(begin + step >= more);
+                            ahead = true;
+                        }
+                    }
+                }
+                wait(&vf[vs.stage], vs.parity, DEV_ERR_FULL_WAIT);
+                const int valid = last_valid - t * kTile;
+                if (ok && valid < kTile) zero_rows(ring + vs.stage * C::STAGE + C::TILE, C::BLOCK, C::BLOCKS, valid, kTile);
+                if (t == begin && results > 0) wait(&o_free[g], (results - 1) & 1u, DEV_ERR_ACC_WAIT);
+                wait(&p_full[g], turns & 1u, DEV_ERR_ACC_WAIT);
                 if (!ok) break;
                 tc_fence_after();
-                umma_bf16_ts_x4<8, 128>(acc, p_at, v_d + (uint64_t)(uint32_t)((st * C::STAGE) >> 4), idesc_o, t > now.t_lo);
+                umma_bf16_ts_x4<8, 128>(o_at, p_at, v_d + (uint64_t)(uint32_t)((vs.stage * C::STAGE) >> 4), idesc_o, t > begin);
                 umma_commit_elect(&o_full[g]);
-                umma_commit_elect(&v_empty[st]);
-            } else if (lane == 0) {
-                mbar_arrive(&v_empty[st]);
+                umma_commit_elect(&ve[vs.stage]);
+                vs.step(part);
             }
-            now.t += step;
+            results += begin < tiles;
         }
     } else if (warp >= 4) {
         // ---- softmax
-        const int g = (warp >> 2) - 1, r = tid & 127;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, buf = tmem + lanes + g * kTile, p_at = tmem + lanes + C::P + g * (kTile / 2), acc = tmem + lanes + C::ACC + g * HD;
+        const int g = (warp >> 2) - 1, r = tid & 127, step = own ? 1 : NG, begin = own ? 0 : g;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + g * kTile, p_at = tmem + C::P + g * (kTile / 2), o_at = tmem + C::ACC + g * HD;
         uint8_t* const mine = smem + C::OUT + (warp - 4) * 2048;
         float2* const stats = (float2*)(smem + C::STATS);
         bool ok = true;
+        // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, DEV_ERR_ACC_WAIT));
-            tc_fence_after();
         };
-        uint32_t turns = 0;  // tiles so far
-        for (int index = 0;; ++index) {
-            take(index, w);
-            if (w.tiles < 0) break;
-            int a_first = 0, a_rows = 0, head = 0, t_lo = 0, t_hi = 0;
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-                if (i == g) {
-                    a_first = w.a_first[i];
-                    a_rows = w.a_rows[i];
-                    head = w.head[i];
-                    t_lo = w.t_lo[i];
-                    t_hi = w.t_hi[i];
-                }
+        uint32_t turns = 0;  // tiles of this group so far
+        for (int index = 0; take(index); ++index) {
             if (own && g >= w.n) continue;
-            const int begin = own ? t_lo : g, step = own ? 1 : NG;
+            int a_first = w.a_first[0], a_rows = w.a_rows[0], head = w.head[0];
+            if (own)
+#pragma unroll
+                for (int i = 1; i < NG; ++i)
+                    if (i == g) {
+                        a_first = w.a_first[i];
+                        a_rows = w.a_rows[i];
+                        head = w.head[i];
+                    }
             const bool live = r < a_rows;
-            const int64_t grow = w.q_first + a_first + r;  // row of the buffers
+            const int grow = w.q_first + a_first + r;  // row of the buffers
             int lo = 0, hi = 0;
             if (live) attn_visible<false>(p, w.q_len, w.k_len, a_first + r, lo, hi);
             float m = -INFINITY, sum = 0.f;
-            for (int t = begin; t < t_hi; t += step, ++turns) {
+            for (int t = begin; t < w.tiles; t += step, ++turns) {
                 const int c_lo = lo - w.first - t * kTile, c_hi = hi - w.first - t * kTile;  // visible columns
                 const bool whole = __all_sync(0xffffffffu, c_lo <= 0 && c_hi >= kTile);
                 wait(&s_full[g], turns & 1u);
+                tc_fence_after();
                 uint32_t s[4][16];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tmem_ld16(buf + k * 16, s[k]);
+                for (int k = 0; k < 4; ++k) tmem_ld16(s_at + lanes + k * 16, s[k]);
                 tc_wait_ld();
                 tc_fence_before();
                 mbar_arrive(&s_free[g]);
@@ -367,10 +349,10 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                     for (int i = 0; i < kTile; ++i)
                         if (i < c_lo || i >= c_hi) s[i >> 4][i & 15] = 0xff800000u;
                 auto at = [&](int i) { return __uint_as_float(s[i >> 4][i & 15]); };
-                float tops[2] = {fmaxf(at(0), at(1)), fmaxf(at(2), at(3))};
+                float tops[4] = {at(0), at(1), at(2), at(3)};
 #pragma unroll
-                for (int i = 4; i < kTile; i += 2) tops[i >> 1 & 1] = max3(tops[i >> 1 & 1], at(i), at(i + 1));
-                const float top = fmaxf(tops[0], tops[1]) * p.scale_log2;  // positive scale: the maximum stays the maximum
+                for (int i = 4; i < kTile; i += 2) tops[i >> 1 & 3] = max3(tops[i >> 1 & 3], at(i), at(i + 1));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * p.scale_log2;  // positive scale: the maximum stays the maximum
                 float corr = 1.f;
                 bool moved = false;
                 if (top > m + 8.f || m == -INFINITY) {
@@ -408,27 +390,31 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                 split2(part[0], parts[0], parts[1]);
                 split2(part[1], parts[2], parts[3]);
                 sum += (parts[0] + parts[1]) + (parts[2] + parts[3]);
-                if (t > begin) wait(&o_full[g], (turns - 1) & 1u);  // the product that read the last P, and wrote O
+                if (t > begin) {  // the product that read the last P, and wrote O
+                    wait(&o_full[g], (turns - 1) & 1u);
+                    tc_fence_after();
+                }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll 1
                     for (int k = 0; k < HD / 16; ++k) {
                         uint32_t o[16];
-                        tmem_ld16(acc + k * 16, o);
+                        tmem_ld16(o_at + lanes + k * 16, o);
                         tc_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-                        tmem_st16(acc + k * 16, o);
+                        tmem_st16(o_at + lanes + k * 16, o);
                     }
                 }
-                tmem_st16(p_at, v[0]);
-                tmem_st16(p_at + 16, v[1]);
+                tmem_st16(p_at + lanes, v[0]);
+                tmem_st16(p_at + lanes + 16, v[1]);
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&p_full[g]);
             }
             // ---- results of the unit
-            const bool any = t_hi > begin;
+            const bool any = begin < w.tiles;
             if (any) wait(&o_full[g], (turns - 1) & 1u);
+            tc_fence_after();
             const int warp_row = (warp & 3) * 32;
             char* const dst = (char*)(p.out0 + (int64_t)(w.q_first + a_first + warp_row) * p.out0_stride + (int64_t)head * p.hd);
             float weight[NG];  // of each group's O
@@ -470,11 +456,11 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                     for (int i = 0; i < 32; ++i) o[i] = fmaf(__uint_as_float(x[i >> 4][i & 15]), f, o[i]);
                 };
                 if (own) {
-                    if (any) add(acc, weight[0]);
+                    if (any) add(o_at + lanes, weight[0]);
                 } else {
 #pragma unroll
                     for (int i = 0; i < NG; ++i)
-                        if (t_hi > i) add(tmem + lanes + C::ACC + i * HD, weight[i]);
+                        if (w.tiles > i) add(tmem + lanes + C::ACC + i * HD, weight[i]);
                 }
                 uint4 v[4];
 #pragma unroll
@@ -497,7 +483,9 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     using C = Cfg<HD>;
     const int G = c.heads / c.kv_heads;
     const int64_t blocks = (c.max_q + kStand - 1) / kStand, all = blocks * c.n_seqs * c.heads;
-    p.parts = all <= kShareUnits * num_sms ? 1 : C::GROUPS;
+    // Units to themselves where every group of every SM gets two, us (one unit at a time against units of their own): 8 ragged x 2 048, 12 heads of 128
+    // 88 against 77; 32 ragged x 512, 14 heads of 64 49 against 41; 1 x 4 096 of them 84 against 88; 1 x 1 000 17 against 37.
+    p.parts = all <= 2 * C::GROUPS * num_sms ? 1 : C::GROUPS;
     const int64_t units = (blocks * G + p.parts - 1) / p.parts * c.n_seqs * c.kv_heads;
     if (units >= 1 << 30 || blocks * G >= 1 << 30) return (int)cudaErrorInvalidValue;
     p.units = (int)units;
