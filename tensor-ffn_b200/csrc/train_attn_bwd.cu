@@ -91,10 +91,10 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* const full = (uint64_t*)(smem + C::BARS);
     uint64_t *const empty = full + C::STAGES, *const a_full = empty + C::STAGES, *const a_empty = a_full + 2, *const s_full = a_empty + 2, *const dp_full = s_full + NG,
-                    *const p_full = dp_full + NG, *const added = p_full + NG, *const acc_done = added + NG, *const acc_free = acc_done + 1, *const u_full = acc_free + 1,
+                    *const p_full = dp_full + NG, *const ds_full = p_full + NG, *const p_added = ds_full + NG, *const ds_added = p_added + NG, *const acc_done = ds_added + NG, *const acc_free = acc_done + 1, *const u_full = acc_free + 1,
                     *const u_empty = u_full + kUnitSlots;
     uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
-    static_assert((2 * C::STAGES + 4 + 4 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 384, "");
+    static_assert((2 * C::STAGES + 4 + 6 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 384, "");
     Unit* const slots = (Unit*)(smem + C::SLOTS);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -110,7 +110,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             mbar_init(&s_full[i], 1);
             mbar_init(&dp_full[i], 1);
             mbar_init(&p_full[i], 128);
-            mbar_init(&added[i], 1);
+            mbar_init(&ds_full[i], 128);
+            mbar_init(&p_added[i], 1);
+            mbar_init(&ds_added[i], 1);
         }
         mbar_init(acc_done, 1);
         mbar_init(acc_free, 4 * NG);
@@ -223,47 +225,89 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             umma_bf16_ts_x4<8, 128>(d, a, n_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4), idesc_acc, more);
         };
         bool ok = true;
-        int item = 0, st = g, turn = 0;  // units with tiles before; stage of the next tile; tiles before, modulo the groups
-        uint32_t parity = 0, mine = 0;   // of the stage; tiles of this group so far
-        for (int index = 0; ok && take(index); ++index) {
-            if (w.tiles == 0) continue;
-            const int ab = item & 1, stream_len = DKV ? w.q_len : w.k_len;
-            int t = g - turn;
-            if (t < 0) t += NG;
-            bool fresh = true;
-            int in_head = t;
-            for (; t < w.tiles && ok; t += NG, ++mine, in_head += NG) {
-                if (fresh) ok = wait(&a_full[ab], (uint32_t)(item >> 1) & 1u, DEV_ERR_FULL_WAIT);
-                fresh = false;
-                if (ok) ok = wait(&full[st], parity, DEV_ERR_FULL_WAIT);
-                if (!ok) break;
-                while (in_head >= w.tiles_per_head) in_head -= w.tiles_per_head;
-                const int valid = stream_len - w.first - in_head * kTile;
-                if (valid < kTile) zero_rows(smem + C::RING + st * C::STAGE, C::BLOCK, 2 * C::BLOCKS, valid, kTile);
-                tc_fence_after();
-                product(buf, 0, ab, st);
-                umma_commit_elect(&s_full[g]);
-                product(buf + kTile, 1, ab, st);
-                umma_commit_elect(&dp_full[g]);
-                ok = wait(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
-                // the results of the unit before have left the accumulators; the tile before has been added
-                if (ok && t == 0 && item > 0) ok = wait(acc_free, (uint32_t)(item - 1) & 1u, DEV_ERR_ACC_WAIT);
-                if (ok && (g > 0 || mine > 0)) ok = wait(&added[before], (g > 0 ? mine : mine - 1) & 1u, DEV_ERR_ACC_WAIT);
-                if (!ok) break;
-                tc_fence_after();
-                accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, st, t > 0);
-                accumulate(tmem + C::ACC + HD, buf + kTile, 0, st, t > 0);
-                umma_commit_elect(&added[g]);
-                umma_commit_elect(&empty[st]);
-                if (t == w.tiles - 1) umma_commit_elect(acc_done);
-                st += NG;
-                if (st >= C::STAGES) {
-                    st -= C::STAGES;
-                    parity ^= 1u;
+        auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
+        // The walk over this group's tiles, which S and dP are at.
+        int index = 0, item = -1, t = 0, in_head = 0, st = 0;  // units taken; units with tiles, less one; the tile in its unit, in its head; its stage
+        uint32_t parity = 0;                       // of the stage
+        bool more = true;
+        w.tiles = 0;
+        // To the next tile, not past `units` more units: a later one waits for results that this warp may owe products to.
+        // False if that is too far, or there is no more.
+        auto find = [&](int units) {
+            while (more && t >= w.tiles) {
+                if (units == 0) return false;
+                t -= w.tiles;
+                more = ok && take(index++);
+                --units;
+                if (!more) w.tiles = 0;
+                if (w.tiles > 0) {
+                    ++item;
+                    // also where this group has no tile: a barrier's parity tells only the next phase from the last one
+                    need(&a_full[item & 1], (uint32_t)(item >> 1) & 1u, DEV_ERR_FULL_WAIT);
                 }
+                in_head = t;
             }
-            turn = (turn + w.tiles) % NG;
-            ++item;
+            return more;
+        };
+        auto advance = [&](int units) {
+            t += NG;
+            in_head += NG;
+            st += NG;
+            if (st >= C::STAGES) {
+                st -= C::STAGES;
+                parity ^= 1u;
+            }
+            return find(units);
+        };
+        // S or dP of the tile that the walk is at; S waits for the tile
+        auto scores = [&](int which) {
+            const int ab = item & 1;
+            if (which == 0) {
+                need(&full[st], parity, DEV_ERR_FULL_WAIT);
+                while (in_head >= w.tiles_per_head) in_head -= w.tiles_per_head;
+                const int valid = (DKV ? w.q_len : w.k_len) - w.first - in_head * kTile;
+                if (ok && valid < kTile) zero_rows(smem + C::RING + st * C::STAGE, C::BLOCK, 2 * C::BLOCKS, valid, kTile);
+                tc_fence_after();
+            }
+            if (!ok) return;
+            product(buf + which * kTile, which, ab, st);
+            umma_commit_elect(which ? &dp_full[g] : &s_full[g]);
+        };
+        t = in_head = st = g;  // the first tile of this group is tile g of all
+        bool have = find(INT32_MAX);
+        if (have) {
+            scores(0);
+            scores(1);
+        }
+        for (uint32_t mine = 0; ok && have; ++mine) {
+            const int at = st, unit = item;
+            const bool first = t == 0, last = t == w.tiles - 1;
+            const uint32_t turns = (g > 0 ? mine : mine - 1) & 1u;  // of the group whose tile is before this one
+            // M += P K or dV += P^T dO, behind the tile before; then S of the next tile in P's place while the group is at dS
+            need(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
+            if (g > 0 || mine > 0) need(&p_added[before], turns, DEV_ERR_ACC_WAIT);
+            // the results of the unit before have left the accumulators (behind the tile before, which has seen those of the unit before that leave)
+            if (first && unit > 0) need(acc_free, (uint32_t)(unit - 1) & 1u, DEV_ERR_ACC_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+            accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
+            umma_commit_elect(&p_added[g]);
+            have = advance(1);
+            const bool early = have;
+            if (early) scores(0);
+            need(&ds_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
+            if (g > 0 || mine > 0) need(&ds_added[before], turns, DEV_ERR_ACC_WAIT);
+            if (!ok) break;
+            tc_fence_after();
+            accumulate(tmem + C::ACC + HD, buf + kTile, 0, at, !first);
+            umma_commit_elect(&ds_added[g]);
+            umma_commit_elect(&empty[at]);
+            if (last) umma_commit_elect(acc_done);
+            if (!early && more) {
+                have = find(INT32_MAX);
+                if (have) scores(0);
+            }
+            if (have) scores(1);
         }
     } else if (warp >= 4) {
         // ---- P and dS
@@ -357,6 +401,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                     weights(std::false_type());
                 else
                     weights(std::true_type());
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[group]);
                 wait(&dp_full[group], ph);
                 F2 part = 0ull;
 #pragma unroll
@@ -389,7 +436,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 }
                 tc_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[group]);
+                mbar_arrive(&ds_full[group]);
             }
             turn = (turn + w.tiles) % NG;
             // ---- results of the unit
