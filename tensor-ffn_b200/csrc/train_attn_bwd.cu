@@ -75,13 +75,14 @@ struct Cfg {
     static constexpr int BLOCKS = HD / 64;                                // column blocks of 64 (128 swizzled bytes)
     static constexpr int BLOCK = kTile * 128, TILE = BLOCKS * BLOCK, STAGE = 2 * TILE;
     static constexpr int A_BLOCK = kStand * 128, A_TILE = BLOCKS * A_BLOCK, A_BYTES = 2 * A_TILE;
-    static constexpr int STAGES = HD == 64 ? 7 : 3;                       // at least one more than groups; what 227 KB hold
-    static constexpr int RING = 2 * A_BYTES, ROWS = RING + STAGES * STAGE, ROWS_BYTES = GROUPS * 2 * kTile * 8;
+    static constexpr int UNITS = HD == 64 ? 2 : 1;                        // units whose standing rows are there: what 227 KB hold next to the ring
+    static constexpr int STAGES = HD == 64 ? 6 : 4;                       // at least two more than groups, for the loads on their way
+    static constexpr int RING = UNITS * A_BYTES, OUT = RING + STAGES * STAGE; // OUT: 2 KB a warp for its results on their way out
+    static constexpr int ROWS = OUT + GROUPS * 4 * 2048, ROWS_BYTES = GROUPS * 2 * kTile * 8;
     static constexpr int SLOTS = ROWS + ROWS_BYTES, BARS = SLOTS + kUnitSlots * (int)sizeof(Unit), SMEM = BARS + 384;
     static constexpr int ACC = GROUPS * 2 * kTile;                        // tensor memory: S and dP of each group, then two accumulators
     static_assert(ACC + 2 * HD <= 512 && SMEM <= 227 * 1024 && STAGES > GROUPS && BARS % 8 == 0, "");
     static_assert(ROWS_BYTES >= GROUPS * kStand * 4, "");                 // the groups' row sums use the same place
-    static_assert(A_BYTES >= GROUPS * 4 * 2048, "");                      // results on their way out use a finished unit's standing rows
 };
 
 template <int HD, bool DKV>
@@ -90,11 +91,11 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     constexpr int NG = C::GROUPS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* const full = (uint64_t*)(smem + C::BARS);
-    uint64_t *const empty = full + C::STAGES, *const a_full = empty + C::STAGES, *const a_empty = a_full + 2, *const s_full = a_empty + 2, *const dp_full = s_full + NG,
+    uint64_t *const empty = full + C::STAGES, *const a_full = empty + C::STAGES, *const a_empty = a_full + C::UNITS, *const s_full = a_empty + C::UNITS, *const dp_full = s_full + NG,
                     *const p_full = dp_full + NG, *const ds_full = p_full + NG, *const p_added = ds_full + NG, *const ds_added = p_added + NG, *const acc_done = ds_added + NG, *const acc_free = acc_done + 1, *const u_full = acc_free + 1,
                     *const u_empty = u_full + kUnitSlots;
     uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
-    static_assert((2 * C::STAGES + 4 + 6 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 384, "");
+    static_assert((2 * C::STAGES + 2 * C::UNITS + 6 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 384, "");
     Unit* const slots = (Unit*)(smem + C::SLOTS);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -102,9 +103,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < C::UNITS; ++i) {
             mbar_init(&a_full[i], 1);
-            mbar_init(&a_empty[i], 4 * NG);  // each warp has stored its results
+            mbar_init(&a_empty[i], NG);  // each group's S and dP are formed
         }
         for (int i = 0; i < NG; ++i) {
             mbar_init(&s_full[i], 1);
@@ -179,8 +180,8 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             __syncwarp();
             if (w.tiles < 0) break;
             if (w.tiles > 0) {
-                const int ab = item & 1;
-                if (item >= 2) ok = wait(&a_empty[ab], (uint32_t)(item / 2 - 1) & 1u);
+                const int ab = item % C::UNITS;
+                if (item >= C::UNITS) ok = wait(&a_empty[ab], (uint32_t)(item / C::UNITS - 1) & 1u);
                 if (!ok) break;
                 mbar_arrive_expect_tx_elect(a_bar + ab * 8, C::A_BYTES);
                 const int a_row = (DKV ? w.k_first : w.q_first) + w.a_first, a_heads = DKV ? p.kv_heads : p.heads;
@@ -226,43 +227,49 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         };
         bool ok = true;
         auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
+        // two at once: a look at a barrier costs 90 cycles even if it is ready
+        auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+            const bool x = mbar_test_wait(a, pa), y = mbar_test_wait(b, pb);
+            if (!__all_sync(0xffffffffu, x && y)) {
+                need(a, pa, DEV_ERR_ACC_WAIT);
+                need(b, pb, DEV_ERR_ACC_WAIT);
+            }
+        };
+        auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)); };
         // The walk over this group's tiles, which S and dP are at.
-        int index = 0, item = -1, t = 0, in_head = 0, st = 0;  // units taken; units with tiles, less one; the tile in its unit, in its head; its stage
-        uint32_t parity = 0;                       // of the stage
+        int index = 0, item = -1, seen = -1;  // units taken; units with tiles, less one; the last of those whose standing rows are known to be there
+        int t = g, in_head = g, st = g;       // the tile in its unit, in its head; its stage. The first tile of this group is tile g of all.
+        uint32_t parity = 0;                  // of the stage
         bool more = true;
         w.tiles = 0;
-        // To the next tile, not past `units` more units: a later one waits for results that this warp may owe products to.
-        // False if that is too far, or there is no more.
+        auto standing = [&]() {
+            if (seen != item) need(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u, DEV_ERR_FULL_WAIT);
+            seen = item;
+        };
+        // To the next tile, not past `units` more units: a later one waits for results that this warp may owe products to. False if that is too
+        // far, or there is no more. A unit's standing rows are left behind: every group sees that they were there, also where it has no tile of the unit, since
+        // a barrier's parity tells only the next phase from the last one.
         auto find = [&](int units) {
             while (more && t >= w.tiles) {
                 if (units == 0) return false;
+                --units;
+                if (w.tiles > 0) {
+                    standing();
+                    umma_commit_elect(&a_empty[item % C::UNITS]);
+                }
                 t -= w.tiles;
                 more = ok && take(index++);
-                --units;
                 if (!more) w.tiles = 0;
-                if (w.tiles > 0) {
-                    ++item;
-                    // also where this group has no tile: a barrier's parity tells only the next phase from the last one
-                    need(&a_full[item & 1], (uint32_t)(item >> 1) & 1u, DEV_ERR_FULL_WAIT);
-                }
+                item += w.tiles > 0;
                 in_head = t;
             }
             return more;
         };
-        auto advance = [&](int units) {
-            t += NG;
-            in_head += NG;
-            st += NG;
-            if (st >= C::STAGES) {
-                st -= C::STAGES;
-                parity ^= 1u;
-            }
-            return find(units);
-        };
-        // S or dP of the tile that the walk is at; S waits for the tile
+        // S or dP of the tile that the walk is at
         auto scores = [&](int which) {
-            const int ab = item & 1;
+            const int ab = item % C::UNITS;
             if (which == 0) {
+                standing();
                 need(&full[st], parity, DEV_ERR_FULL_WAIT);
                 while (in_head >= w.tiles_per_head) in_head -= w.tiles_per_head;
                 const int valid = (DKV ? w.q_len : w.k_len) - w.first - in_head * kTile;
@@ -273,7 +280,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             product(buf + which * kTile, which, ab, st);
             umma_commit_elect(which ? &dp_full[g] : &s_full[g]);
         };
-        t = in_head = st = g;  // the first tile of this group is tile g of all
         bool have = find(INT32_MAX);
         if (have) {
             scores(0);
@@ -281,32 +287,41 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         }
         for (uint32_t mine = 0; ok && have; ++mine) {
             const int at = st, unit = item;
-            const bool first = t == 0, last = t == w.tiles - 1;
+            const bool first = t == 0, last = t == w.tiles - 1, follows = g > 0 || mine > 0;
             const uint32_t turns = (g > 0 ? mine : mine - 1) & 1u;  // of the group whose tile is before this one
+            t += NG;
+            in_head += NG;
+            st += NG;
+            if (st >= C::STAGES) {
+                st -= C::STAGES;
+                parity ^= 1u;
+            }
+            have = find(1);
             // M += P K or dV += P^T dO, behind the tile before; then S of the next tile in P's place while the group is at dS
-            need(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
-            if (g > 0 || mine > 0) need(&p_added[before], turns, DEV_ERR_ACC_WAIT);
+            if (follows)
+                need_both(&p_full[g], mine & 1u, &p_added[before], turns);
+            else
+                need(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
             // the results of the unit before have left the accumulators (behind the tile before, which has seen those of the unit before that leave)
             if (first && unit > 0) need(acc_free, (uint32_t)(unit - 1) & 1u, DEV_ERR_ACC_WAIT);
             if (!ok) break;
             tc_fence_after();
             accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
             umma_commit_elect(&p_added[g]);
-            have = advance(1);
-            const bool early = have;
+            const bool early = have && (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity);
             if (early) scores(0);
-            need(&ds_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
-            if (g > 0 || mine > 0) need(&ds_added[before], turns, DEV_ERR_ACC_WAIT);
+            if (follows)
+                need_both(&ds_full[g], mine & 1u, &ds_added[before], turns);
+            else
+                need(&ds_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
             if (!ok) break;
             tc_fence_after();
             accumulate(tmem + C::ACC + HD, buf + kTile, 0, at, !first);
             umma_commit_elect(&ds_added[g]);
             umma_commit_elect(&empty[at]);
             if (last) umma_commit_elect(acc_done);
-            if (!early && more) {
-                have = find(INT32_MAX);
-                if (have) scores(0);
-            }
+            if (!have && more) have = find(INT32_MAX);
+            if (have && !early) scores(0);
             if (have) scores(1);
         }
     } else if (warp >= 4) {
@@ -386,8 +401,12 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                                 const int c = half * 32 + i + e, k = i + e;
                                 float x, y;
                                 split2(fma2(f2(__uint_as_float(s[k >> 4][k & 15]), __uint_as_float(s[k >> 4][(k & 15) + 1])), scale2, e ? f2(l4.z, l4.w) : f2(l4.x, l4.y)), x, y);
-                                x = exp2_fast(x);
-                                y = exp2_fast(y);
+                                if (HD == 64 && !masked.value && k % 8 == 6) {
+                                    split2(exp2_poly(f2(x, y)), x, y);
+                                } else {
+                                    x = exp2_fast(x);
+                                    y = exp2_fast(y);
+                                }
                                 if (masked.value && (c < c_lo || c >= c_hi)) x = 0.f;
                                 if (masked.value && (c + 1 < c_lo || c + 1 >= c_hi)) y = 0.f;
                                 pr[c >> 1] = f2(x, y);
@@ -453,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 }
             }
             // 64 bytes of a row at a time, dealt to the groups: 32 columns, or 16 of an fp32 sum
-            uint8_t* const out = smem + (item & 1) * C::A_BYTES + (warp - 4) * 2048;  // the unit's standing rows have been read for the last time
+            uint8_t* const out = smem + C::OUT + (warp - 4) * 2048;
             const int warp_row = (warp & 3) * 32, rows = w.a_rows - warp_row, grow0 = grow - (r & 31);
             bool freed = false;
             auto free_sums = [&]() {  // this warp's last look at the accumulators
@@ -509,9 +528,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 else
                     store(std::false_type());
                 if (!freed) free_sums();
-                fence_proxy_async_smem();  // the next standing rows come through the other proxy
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&a_empty[item & 1]);
                 ++item;
             } else if (live) {  // nothing is seen: zeros
                 for (int k = group; k < (DKV ? 2 : 1) * p.hd / 8; k += NG) {
