@@ -230,8 +230,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
         // two at once: a barrier that is ready costs 90 cycles to look at
         auto wait_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
-            const bool x = mbar_test_wait(a, pa), y = mbar_test_wait(b, pb);
-            if (!__all_sync(0xffffffffu, x && y)) {
+            if (!__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
                 wait(a, pa, DEV_ERR_FULL_WAIT);
                 wait(b, pb, DEV_ERR_ACC_WAIT);
             }

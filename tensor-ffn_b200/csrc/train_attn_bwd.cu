@@ -227,10 +227,10 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         };
         bool ok = true;
         auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
-        // two at once: a look at a barrier costs 90 cycles even if it is ready
+        // Two of them. A look at a barrier costs 90 cycles even if it is ready, so both at once where that is likely; beside three groups the
+        // looks in vain cost more than they save (8 x 4 096, 64 columns: 1 200 us, else 1 100; 1 x 8 192, 128 columns: 1 730, else 1 790).
         auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
-            const bool x = mbar_test_wait(a, pa), y = mbar_test_wait(b, pb);
-            if (!__all_sync(0xffffffffu, x && y)) {
+            if (HD == 64 || !__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
                 need(a, pa, DEV_ERR_ACC_WAIT);
                 need(b, pb, DEV_ERR_ACC_WAIT);
             }
@@ -296,7 +296,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 st -= C::STAGES;
                 parity ^= 1u;
             }
-            have = find(1);
             // M += P K or dV += P^T dO, behind the tile before; then S of the next tile in P's place while the group is at dS
             if (follows)
                 need_both(&p_full[g], mine & 1u, &p_added[before], turns);
@@ -308,7 +307,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             tc_fence_after();
             accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
             umma_commit_elect(&p_added[g]);
-            const bool early = have && (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity);
+            have = find(1);
+            // 64 columns: six stages, the tile is as good as there; 128: four, dS comes first where it is not
+            const bool early = have && ((HD == 64 && seen == item) || (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity));
             if (early) scores(0);
             if (follows)
                 need_both(&ds_full[g], mine & 1u, &ds_added[before], turns);
@@ -401,12 +402,8 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                                 const int c = half * 32 + i + e, k = i + e;
                                 float x, y;
                                 split2(fma2(f2(__uint_as_float(s[k >> 4][k & 15]), __uint_as_float(s[k >> 4][(k & 15) + 1])), scale2, e ? f2(l4.z, l4.w) : f2(l4.x, l4.y)), x, y);
-                                if (HD == 64 && !masked.value && k % 8 == 6) {
-                                    split2(exp2_poly(f2(x, y)), x, y);
-                                } else {
-                                    x = exp2_fast(x);
-                                    y = exp2_fast(y);
-                                }
+                                x = exp2_fast(x);
+                                y = exp2_fast(y);
                                 if (masked.value && (c < c_lo || c >= c_hi)) x = 0.f;
                                 if (masked.value && (c + 1 < c_lo || c + 1 >= c_hi)) y = 0.f;
                                 pr[c >> 1] = f2(x, y);
@@ -548,27 +545,39 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
-// D'[h][row] = sum of dO o O over the head: L = HD / 8 lanes a row, neighbouring rows in neighbouring lanes
+// D'[h][row] = sum of dO o O over the head: L = HD / 8 lanes a row, neighbouring rows in neighbouring lanes, four rows a lane in flight
 template <int L>
 __global__ void __launch_bounds__(256) k_attn_dot(const bf16* __restrict__ d_out, const bf16* __restrict__ out, int64_t stride, const int* cu_q, int n_seqs, int64_t rows, int heads,
                                                   int hd, float* __restrict__ d) {
+    constexpr int ROWS = 256 / L;
     pdl_launch_dependents();
-    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int64_t row0 = (int64_t)blockIdx.x * (4 * ROWS) + threadIdx.x / L;
     const int h = blockIdx.y, c = threadIdx.x % L * 8;
-    const bool live = row < rows && row >= cu_q[0] && row < cu_q[n_seqs];
-    float a = 0.f;
-    if (live && c < hd) {
-        const uint4 x = __ldg((const uint4*)(d_out + row * stride + (int64_t)h * hd + c)), y = __ldg((const uint4*)(out + row * stride + (int64_t)h * hd + c));
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    const int64_t begin = max(cu_q[0], 0), end = min((int64_t)cu_q[n_seqs], rows);
+    uint4 x[4], y[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a = fmaf(bf16_lo(xs[i]), bf16_lo(ys[i]), a);
-            a = fmaf(bf16_hi(xs[i]), bf16_hi(ys[i]), a);
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + i * ROWS;
+        x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row >= begin && row < end && c < hd) {
+            x[i] = __ldg((const uint4*)(d_out + row * stride + (int64_t)h * hd + c));
+            y[i] = __ldg((const uint4*)(out + row * stride + (int64_t)h * hd + c));
         }
     }
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-    if (live && c == 0) d[(int64_t)h * rows + row] = a;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = row0 + i * ROWS;
+        const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+        float a = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a = fmaf(bf16_lo(xs[k]), bf16_lo(ys[k]), a);
+            a = fmaf(bf16_hi(xs[k]), bf16_hi(ys[k]), a);
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (row >= begin && row < end && c == 0) d[(int64_t)h * rows + row] = a;
+    }
 }
 
 // dK and dV from the parts of the query heads, added in their order
@@ -642,7 +651,7 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
     int rc = 0;
     if (queries) {
         const int lanes = c.hd <= 64 ? 8 : 16;
-        const dim3 grid((unsigned)((c.rows_q + 256 / lanes - 1) / (256 / lanes)), (unsigned)c.heads);
+        const dim3 grid((unsigned)((c.rows_q + 1024 / lanes - 1) / (1024 / lanes)), (unsigned)c.heads);
         rc = lanes == 8 ? (int)launch_k(k_attn_dot<8>, grid, dim3(256), 0, s, false, c.d_out, (const bf16*)c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d)
                         : (int)launch_k(k_attn_dot<16>, grid, dim3(256), 0, s, false, c.d_out, (const bf16*)c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d);
         if (rc) return rc;
