@@ -8,8 +8,9 @@
 //
 // Bound by HBM: logits are read once and gradients written once. A row of a 151 936-word vocabulary is 608 KB, so a thread-block cluster
 // holds it in its shared memory between the sum and the gradient: each block one slice, fetched by bulk copies in pieces of 16 KB that
-// are summed as they land; the blocks exchange (maximum, sum, x[y]) through distributed shared memory. Slices of about 100 KB leave two
-// blocks an SM, so that one row's copies run under another's arithmetic and stores.
+// are summed as they land; the blocks exchange (maximum, sum, x[y]) through distributed shared memory. Slices of 76 KB leave three
+// blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 434 us,
+// 5.0 TB/s; two slices of 101 KB 460 us).
 #include "launch.h"
 #include "ptx.cuh"
 #include "train.h"
@@ -23,7 +24,7 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPiece = 16384;              // bytes of a bulk copy
 constexpr int kMaxSlice = 216 * 1024;      // bytes of a row that one block can hold
-constexpr int kSharedSlice = 108 * 1024;   // the same with two blocks an SM
+constexpr int kPerSm = 3, kSharedSlice = (228 * 1024 / kPerSm - 1024 - 600) / 16 * 16;  // the same with three blocks an SM
 constexpr int kMaxBlocks = 8;              // blocks of a cluster
 constexpr int kMaxPieces = (kMaxSlice + kPiece - 1) / kPiece;
 constexpr int kHead = 256;                 // barriers and the blocks' partial results, in front of the slice
@@ -123,21 +124,37 @@ __device__ __forceinline__ Lse block_join(Lse l, float (*slot)[2]) {
     return all;
 }
 
-// sums of a cluster's blocks joined in rank order, and x[y] in base 2; the same numbers in every block
+// sums of a cluster's blocks joined in a fixed order, and x[y]; the same numbers in every lane of the calling warp and in every block. Lane = block, so that the
+// loads from the others' shared memory are on their way together.
 struct RowSum {
     Lse rest;      // everything but the token
     float token;   // its logit
 };
 __device__ __forceinline__ RowSum cluster_join(const float* mine, uint32_t blocks) {
+    const uint32_t lane = threadIdx.x & 31;
     RowSum r;
-    r.token = -INFINITY;
-    for (uint32_t i = 0; i < blocks; ++i) {
-        const uint32_t peer = blocks > 1 ? map_shared_rank(smem_u32(mine), i) : 0;
-        const float m = blocks > 1 ? ld_shared_cluster_f32(peer) : mine[0], s = blocks > 1 ? ld_shared_cluster_f32(peer + 4) : mine[1];
-        const float x = blocks > 1 ? ld_shared_cluster_f32(peer + 8) : mine[2], has = blocks > 1 ? ld_shared_cluster_f32(peer + 12) : mine[3];
-        r.rest.join(m, s);
-        if (has != 0.f) r.token = x;
+    r.token = 0.f;
+    float has = 0.f;
+    if (lane < blocks) {
+        if (blocks > 1) {
+            const uint32_t peer = map_shared_rank(smem_u32(mine), lane);
+            r.rest.m = ld_shared_cluster_f32(peer);
+            r.rest.s = ld_shared_cluster_f32(peer + 4);
+            r.token = ld_shared_cluster_f32(peer + 8);
+            has = ld_shared_cluster_f32(peer + 12);
+        } else {
+            r.rest.m = mine[0];
+            r.rest.s = mine[1];
+            r.token = mine[2];
+            has = mine[3];
+        }
     }
+    const unsigned owner = __ballot_sync(0xffffffffu, has != 0.f);
+    r.token = owner ? __shfl_sync(0xffffffffu, r.token, __ffs(owner) - 1) : -INFINITY;
+#pragma unroll
+    for (int o = kMaxBlocks / 2; o > 0; o >>= 1) r.rest.join(__shfl_xor_sync(0xffffffffu, r.rest.m, o), __shfl_xor_sync(0xffffffffu, r.rest.s, o));
+    r.rest.m = __shfl_sync(0xffffffffu, r.rest.m, 0);
+    r.rest.s = __shfl_sync(0xffffffffu, r.rest.s, 0);
     return r;
 }
 // log of S / exp(x[y]); -inf where nothing but the token weighs. In logarithms, since a masked token's logit may be the type's lowest value
@@ -193,10 +210,13 @@ __global__ void __launch_bounds__(THREADS) k_token_logprobs(const T* __restrict_
         mine[2] = has ? load_one(src + y) : 0.f;
         mine[3] = has ? 1.f : 0.f;
     }
-    if (blocks > 1) cluster_sync_all();
-    if (rank == 0 && threadIdx.x == 0) {
+    if (blocks > 1)
+        cluster_sync_all();
+    else
+        __syncwarp();
+    if (rank == 0 && threadIdx.x < 32) {
         const RowSum r = cluster_join(mine, blocks);
-        logprob[row] = (unsigned)y < (unsigned)vocab ? (float)token_logprob(log_odds_against(r)) : 0.f;
+        if (threadIdx.x == 0) logprob[row] = (unsigned)y < (unsigned)vocab ? (float)token_logprob(log_odds_against(r)) : 0.f;
     }
     if (blocks > 1) cluster_sync_all();  // the others' results have been read
 }
@@ -216,7 +236,7 @@ struct PolicyDev {
 
 // WIDE: rows start on 16 bytes. One cluster per row.
 template <typename T, int THREADS, bool WIDE>
-__global__ void __launch_bounds__(THREADS) k_policy_loss(const __grid_constant__ PolicyDev p) {
+__global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_loss(const __grid_constant__ PolicyDev p) {
     using P = Pack<T>;
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* const landed = (uint64_t*)smem;  // one barrier a piece
@@ -288,8 +308,11 @@ __global__ void __launch_bounds__(THREADS) k_policy_loss(const __grid_constant__
         mine[2] = has ? load_one(x_s + (y - begin)) : 0.f;
         mine[3] = has ? 1.f : 0.f;
     }
-    if (blocks > 1) cluster_sync_all();
-    if (tid == 0) {
+    if (blocks > 1)
+        cluster_sync_all();
+    else
+        __syncwarp();
+    if (tid < 32) {
         const RowSum r = cluster_join(mine, blocks);
         const double log_odds = log_odds_against(r), lp = token_logprob(log_odds);
         const double adv = p.advantage[row], ratio = exp(lp - (double)p.old_logprob[row]), away = p.ref_logprob ? (double)p.ref_logprob[row] - lp : 0.0;
@@ -299,10 +322,12 @@ __global__ void __launch_bounds__(THREADS) k_policy_loss(const __grid_constant__
         // p[j] = 2^(x[j] log2 e - top) * share, top the larger of the two exponents so that nothing overflows
         const float token = r.token * kLog2e, top = fmaxf(r.rest.m, token);
         const double share = 1.0 / ((double)r.rest.s * exp2((double)r.rest.m - (double)top) + exp2((double)r.token * (double)kLog2e - (double)top));
-        coef[0] = top;
-        coef[1] = (float)(-slope * share);
-        coef[2] = (float)(slope / (1.0 + exp(-log_odds)));  // of the token: 1 - p[y]
-        if (rank == 0) {
+        if (tid == 0) {
+            coef[0] = top;
+            coef[1] = (float)(-slope * share);
+            coef[2] = (float)(slope / (1.0 + exp(-log_odds)));  // of the token: 1 - p[y]
+        }
+        if (rank == 0 && tid == 0) {
             if (p.logprob) p.logprob[row] = (float)lp;
             if (p.row_loss) p.row_loss[row] = (float)((double)weight * ((double)p.kl_coef * kl - fmin(free, clipped)));
             if (p.kl) p.kl[row] = (float)kl;
@@ -351,7 +376,7 @@ __global__ void __launch_bounds__(1024) k_loss_sum(const float* row_loss, int64_
 // elements of a block's slice: an equal share, in whole 16-byte packs
 int slice_of(int vocab, int blocks, int per_pack) { return ((vocab + blocks - 1) / blocks + per_pack - 1) / per_pack * per_pack; }
 
-// Blocks of a row. Two slices fit an SM where the row allows it; with fewer rows than SMs a row is cut further, to pieces of 8 KB, so that
+// Blocks of a row. Three slices fit an SM where the row allows it; with fewer rows than SMs a row is cut further, to pieces of 8 KB, so that
 // more SMs fetch it.
 int blocks_of(int64_t bytes, int64_t rows, int num_sms, int64_t hold) {
     int64_t n = (bytes + hold - 1) / hold;
