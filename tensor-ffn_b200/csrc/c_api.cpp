@@ -4,6 +4,8 @@
 #include "../../include/tffn_diag.h"
 #include "engine.h"
 #include "train.h"
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -428,23 +430,23 @@ void* tffn_session_stream(const tffn_session* s) { return s ? (void*)s->s->strea
 namespace {
 
 struct OnDevice {
-    int before = -1, num_sms = 0;
-    explicit OnDevice(int device) {
-        int n = 0;
-        if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
-            cudaGetLastError();
-            throw Error(kErrCuda, "no CUDA device is available");
-        }
-        need(device >= 0 && device < n, "no such device");
+    int before = -1, device, num_sms = 0;
+    explicit OnDevice(int dev) : device(dev) {
+        static const int count = tffn_device_count();
+        static std::atomic<int> sms[64];
+        if (count == 0) throw Error(kErrCuda, "no CUDA device is available");
+        need(device >= 0 && device < count && device < 64, "no such device");
         TFFN_CUDA(cudaGetDevice(&before));
-        TFFN_CUDA(cudaSetDevice(device));
-        const cudaError_t e = cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device);
-        if (e != cudaSuccess) {
-            cudaSetDevice(before);
-            cuda_check(e, "cudaDeviceGetAttribute", __FILE__, __LINE__);
+        num_sms = sms[device].load(std::memory_order_relaxed);
+        if (num_sms == 0) {
+            TFFN_CUDA(cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, device));
+            sms[device].store(num_sms, std::memory_order_relaxed);
         }
+        if (before != device) TFFN_CUDA(cudaSetDevice(device));
     }
-    ~OnDevice() { cudaSetDevice(before); }
+    ~OnDevice() {
+        if (before != device) cudaSetDevice(before);
+    }
     OnDevice(const OnDevice&) = delete;
 };
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
