@@ -571,6 +571,7 @@ int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const vo
         c.dbias = dbias;
         c.workspace = (float*)workspace;
         OnDevice on(device);
+        c.status = status_word(device);
         check_launch(launch_norm_backward(c, on.num_sms, (cudaStream_t)stream), "norm backward");
     });
 }

@@ -42,6 +42,7 @@ struct NormCall {
     void* dx;
     float *dweight, *dbias;  // or nullptr
     float* workspace;        // norm_workspace_floats, unless dweight and dbias are nullptr
+    int* status;
 };
 constexpr int kNormMaxWidth = 16384;
 int64_t norm_workspace_floats(int64_t rows, int width);
