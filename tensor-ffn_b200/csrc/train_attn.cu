@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
     // a reader's copy of the index-th units of the block; false if there are no more
     auto take = [&](int index) {
         const int slot = index % kUnitSlots;
-        const bool there = __all_sync(0xffffffffu, mbar_wait(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
+        const bool there = __all_sync(0xffffffffu, wait_barrier(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
         w = slots[slot];
         __syncwarp();
         if (lane == 0) mbar_arrive(&u_empty[slot]);
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
     if (warp == 0) {
         // ---- units, and by TMA their queries, then keys and values tile by tile
         const uint32_t base = smem_u32(smem);
-        auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
+        auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait_barrier(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
         bool ok = true;
         int begun[NG] = {0};
         Place fill[NG];
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         uint64_t *const kf = k_full + ring0, *const ke = k_empty + ring0, *const vf = v_full + ring0, *const ve = v_empty + ring0;
         const uint64_t q_d = umma_desc_k128(base + qb * C::Q_TILE), k_d = umma_desc_k128(smem_u32(ring)), v_d = umma_desc_n128(smem_u32(ring) + C::TILE, C::BLOCK);
         bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, code)); };
         // two at once: a barrier that is ready costs 90 cycles to look at
         auto wait_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
             if (!__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         bool ok = true;
         // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, DEV_ERR_ACC_WAIT));
+            if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
         };
         uint32_t turns = 0;  // tiles of this group so far
         for (int index = 0; take(index); ++index) {

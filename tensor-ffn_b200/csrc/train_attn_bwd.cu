@@ -17,10 +17,13 @@
 // of dK, dV: 8 products of a tile instead of 5 (6 with the exact D), but no sum of dQ through memory.
 //
 // A persistent block of three (64 columns a head) or two (128) groups of four warps, thread = standing row, so that a row's mask is an interval of
-// columns; the groups take turns at the tiles, one's exponentials under the others' products. One warp works out the units and fills the
-// rings by TMA; one per group issues its products. The sums of all tiles go to the same accumulators: the product warps take turns at
-// them, each waiting for the one before, so that a row is always added up in one order. The warps run on into the next unit of work while the
-// last one's results are stored.
+// columns; the groups take turns at the tiles, one's exponentials under the others' products. Four more warps turn the accumulators into results
+// while the groups are at the next unit. One warp works out the units and fills the rings by TMA; one per group issues its products. The sums of all tiles go to the same accumulators: the product warps take turns at
+// them, each waiting for the one before, so that a row is always added up in one order.
+//
+// All these programs run at once, and short sequences go through all of their code all the time: what does not fit the instruction cache
+// is what such a call waits for (32 sequences of up to 512 queries, 14 / 2 heads of 64 columns: 112 us; with a mask variant of P and
+// unrolled waits 157 us; then with the results in the groups' hands 152 us).
 #include "train_attn.cuh"
 #include <cstring>
 #include <type_traits>
@@ -30,6 +33,12 @@ namespace tffn {
 namespace {
 
 constexpr int kTile = 64;
+
+// registers of a thread of this warp and its three neighbours from here on; all four come here
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // 128 standing rows of one head (of one kv head and some of its query heads for dK, dV) and the streamed rows that any of them sees
 struct Unit {
@@ -71,18 +80,18 @@ __device__ __forceinline__ void unit_of(const AttnDev& p, const AttnUnit& u, Uni
 
 template <int HD>
 struct Cfg {
-    static constexpr int GROUPS = HD == 64 ? 3 : 2, THREADS = (4 * GROUPS + 4) * 32;
+    static constexpr int GROUPS = HD == 64 ? 3 : 2, THREADS = (4 * GROUPS + 8) * 32;
     static constexpr int BLOCKS = HD / 64;                                // column blocks of 64 (128 swizzled bytes)
     static constexpr int BLOCK = kTile * 128, TILE = BLOCKS * BLOCK, STAGE = 2 * TILE;
     static constexpr int A_BLOCK = kStand * 128, A_TILE = BLOCKS * A_BLOCK, A_BYTES = 2 * A_TILE;
     static constexpr int UNITS = HD == 64 ? 2 : 1;                        // units whose standing rows are there: what 227 KB hold next to the ring
     static constexpr int STAGES = HD == 64 ? 6 : 4;                       // at least two more than groups, for the loads on their way
-    static constexpr int RING = UNITS * A_BYTES, OUT = RING + STAGES * STAGE; // OUT: 2 KB a warp for its results on their way out
-    static constexpr int ROWS = OUT + GROUPS * 4 * 2048, ROWS_BYTES = GROUPS * 2 * kTile * 8;
-    static constexpr int SLOTS = ROWS + ROWS_BYTES, BARS = SLOTS + kUnitSlots * (int)sizeof(Unit), SMEM = BARS + 384;
+    static constexpr int RING = UNITS * A_BYTES, OUT = RING + STAGES * STAGE; // OUT: 2 KB a warp for results on their way out
+    static constexpr int ROWS = OUT + 4 * 2048, ROWS_BYTES = GROUPS * 2 * kTile * 8;
+    static constexpr int SLOTS = ROWS + ROWS_BYTES, BARS = SLOTS + kUnitSlots * (int)sizeof(Unit), SMEM = BARS + 448;
     static constexpr int ACC = GROUPS * 2 * kTile;                        // tensor memory: S and dP of each group, then two accumulators
     static_assert(ACC + 2 * HD <= 512 && SMEM <= 227 * 1024 && STAGES > GROUPS && BARS % 8 == 0, "");
-    static_assert(ROWS_BYTES >= GROUPS * kStand * 4, "");                 // the groups' row sums use the same place
+    static_assert(ROWS_BYTES >= 2 * GROUPS * kStand * 4, "");             // the groups' row sums of two units use the same place
 };
 
 template <int HD, bool DKV>
@@ -92,10 +101,11 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* const full = (uint64_t*)(smem + C::BARS);
     uint64_t *const empty = full + C::STAGES, *const a_full = empty + C::STAGES, *const a_empty = a_full + C::UNITS, *const s_full = a_empty + C::UNITS, *const dp_full = s_full + NG,
-                    *const p_full = dp_full + NG, *const ds_full = p_full + NG, *const p_added = ds_full + NG, *const ds_added = p_added + NG, *const acc_done = ds_added + NG, *const acc_free = acc_done + 1, *const u_full = acc_free + 1,
+                    *const p_full = dp_full + NG, *const ds_full = p_full + NG, *const p_added = ds_full + NG, *const ds_added = p_added + NG, *const acc_done = ds_added + NG, *const acc_free = acc_done + 1, *const sum_full = acc_free + 1, *const sum_empty = sum_full + 2,
+                    *const u_full = sum_empty + 2,
                     *const u_empty = u_full + kUnitSlots;
     uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
-    static_assert((2 * C::STAGES + 2 * C::UNITS + 6 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 384, "");
+    static_assert((2 * C::STAGES + 2 * C::UNITS + 6 * NG + 6 + 2 * kUnitSlots) * 8 + 4 <= 448, "");
     Unit* const slots = (Unit*)(smem + C::SLOTS);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -116,10 +126,14 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             mbar_init(&ds_added[i], 1);
         }
         mbar_init(acc_done, 1);
-        mbar_init(acc_free, 4 * NG);
+        mbar_init(acc_free, 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sum_full[i], 4 * NG);
+            mbar_init(&sum_empty[i], 4);
+        }
         for (int i = 0; i < kUnitSlots; ++i) {
             mbar_init(&u_full[i], 1);
-            mbar_init(&u_empty[i], NG + 4 * NG);
+            mbar_init(&u_empty[i], NG + 4 * NG + 4);
         }
         fence_mbar_init();
     }
@@ -154,7 +168,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     // a reader's copy of the index-th unit of the block
     auto take = [&](int index) {
         const int slot = index % kUnitSlots;
-        const bool there = __all_sync(0xffffffffu, mbar_wait(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
+        const bool there = __all_sync(0xffffffffu, wait_barrier(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
         w = slots[slot];
         if (!there) w.tiles = -1;
         __syncwarp();
@@ -162,179 +176,180 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         return w.tiles >= 0;
     };
 
-    if (warp == 0) {
-        // ---- units, and by TMA their standing rows, then their tiles
-        const uint32_t base = smem_u32(smem), bar = smem_u32(full), a_bar = smem_u32(a_full);
-        auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
-        bool ok = true;
-        int item = 0, st = 0;
-        uint32_t round = 0;
-        for (int index = 0; ok; ++index) {
-            const int slot = index % kUnitSlots;
-            if (index >= kUnitSlots) ok = wait(&u_empty[slot], (uint32_t)(index / kUnitSlots - 1) & 1u);
-            if (!ok) break;
-            if (lane == 0) {
-                slots[slot] = w;
-                mbar_arrive(&u_full[slot]);
-            }
-            __syncwarp();
-            if (w.tiles < 0) break;
-            if (w.tiles > 0) {
-                const int ab = item % C::UNITS;
-                if (item >= C::UNITS) ok = wait(&a_empty[ab], (uint32_t)(item / C::UNITS - 1) & 1u);
+    // 640 threads of 96 registers (64 columns a head), dealt out again: 4 * (48 + 3 * 120 + 72) = 20 * 96 a lane
+    if (warp < 4) {
+        if (HD == 64) reg_dec<48>();
+        if (warp == 0) {
+            // ---- units, and by TMA their standing rows, then their tiles
+            const uint32_t base = smem_u32(smem), bar = smem_u32(full), a_bar = smem_u32(a_full);
+            auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait_barrier(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
+            bool ok = true;
+            int item = 0, st = 0;
+            uint32_t round = 0;
+            for (int index = 0; ok; ++index) {
+                const int slot = index % kUnitSlots;
+                if (index >= kUnitSlots) ok = wait(&u_empty[slot], (uint32_t)(index / kUnitSlots - 1) & 1u);
                 if (!ok) break;
-                mbar_arrive_expect_tx_elect(a_bar + ab * 8, C::A_BYTES);
-                const int a_row = (DKV ? w.k_first : w.q_first) + w.a_first, a_heads = DKV ? p.kv_heads : p.heads;
-                load_head<C::BLOCKS>(&p.tmA[0], base + ab * C::A_BYTES, C::A_BLOCK, a_heads, w.head, a_row, a_bar + ab * 8);
-                load_head<C::BLOCKS>(&p.tmA[1], base + ab * C::A_BYTES + C::A_TILE, C::A_BLOCK, a_heads, w.head, a_row, a_bar + ab * 8);
-                ++item;
-            }
-            int h = w.h0, t = 0;
-            for (int j = 0; j < w.tiles && ok; ++j) {
-                if (round > 0) ok = wait(&empty[st], (round - 1) & 1u);
-                if (!ok) break;
-                const uint32_t b = bar + st * 8, dst = base + C::RING + st * C::STAGE;
-                mbar_arrive_expect_tx_elect(b, C::STAGE);
-                const int row = (DKV ? w.q_first : w.k_first) + w.first + t * kTile;
-                load_head<C::BLOCKS>(&p.tm[0], dst, C::BLOCK, DKV ? p.heads : p.kv_heads, DKV ? h : w.kvh, row, b);
-                load_head<C::BLOCKS>(&p.tm[1], dst + C::TILE, C::BLOCK, DKV ? p.heads : p.kv_heads, DKV ? h : w.kvh, row, b);
-                if (++t == w.tiles_per_head) {
-                    t = 0;
-                    ++h;
+                if (lane == 0) {
+                    slots[slot] = w;
+                    mbar_arrive(&u_full[slot]);
                 }
-                if (++st == C::STAGES) {
-                    st = 0;
-                    ++round;
-                }
-            }
-            if (ok) next();
-        }
-    } else if (warp <= NG) {
-        // ---- products of one group
-        const int g = warp - 1, before = g == 0 ? NG - 1 : g - 1;
-        constexpr uint32_t idesc_s = umma_idesc_bf16(kStand, kTile), idesc_acc = umma_idesc_bf16(kStand, HD) | (1u << 16);  // streamed tile: its K extent in rows
-        const uint32_t base = smem_u32(smem), buf = tmem + g * 2 * kTile;
-        const uint64_t a_d = umma_desc_k128(base), k_d = umma_desc_k128(base + C::RING), n_d = umma_desc_n128(base + C::RING, C::BLOCK);
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, code)); };
-        auto product = [&](uint32_t d, int which, int ab, int st) {
-            const uint64_t a = a_d + (uint64_t)(uint32_t)((ab * C::A_BYTES + which * C::A_TILE) >> 4), b = k_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4);
-#pragma unroll
-            for (int i = 0; i < C::BLOCKS; ++i) umma_bf16_x4<2, 2>(d, a + i * (C::A_BLOCK >> 4), b + i * (C::BLOCK >> 4), idesc_s, i > 0);
-        };
-        auto accumulate = [&](uint32_t d, uint32_t a, int which, int st, bool more) {
-            static_assert(kTile == 64, "four products of 16 rows");
-            umma_bf16_ts_x4<8, 128>(d, a, n_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4), idesc_acc, more);
-        };
-        bool ok = true;
-        auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
-        // Two of them. A look at a barrier costs 90 cycles even if it is ready, so both at once where that is likely; beside three groups the
-        // looks in vain cost more than they save (8 x 4 096, 64 columns: 1 200 us, else 1 100; 1 x 8 192, 128 columns: 1 730, else 1 790).
-        auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
-            if (HD == 64 || !__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
-                need(a, pa, DEV_ERR_ACC_WAIT);
-                need(b, pb, DEV_ERR_ACC_WAIT);
-            }
-        };
-        auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)); };
-        // The walk over this group's tiles, which S and dP are at.
-        int index = 0, item = -1, seen = -1;  // units taken; units with tiles, less one; the last of those whose standing rows are known to be there
-        int t = g, in_head = g, st = g;       // the tile in its unit, in its head; its stage. The first tile of this group is tile g of all.
-        uint32_t parity = 0;                  // of the stage
-        bool more = true;
-        w.tiles = 0;
-        auto standing = [&]() {
-            if (seen != item) need(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u, DEV_ERR_FULL_WAIT);
-            seen = item;
-        };
-        // To the next tile, not past `units` more units: a later one waits for results that this warp may owe products to. False if that is too
-        // far, or there is no more. A unit's standing rows are left behind: every group sees that they were there, also where it has no tile of the unit, since
-        // a barrier's parity tells only the next phase from the last one.
-        auto find = [&](int units) {
-            while (more && t >= w.tiles) {
-                if (units == 0) return false;
-                --units;
+                __syncwarp();
+                if (w.tiles < 0) break;
                 if (w.tiles > 0) {
-                    standing();
-                    umma_commit_elect(&a_empty[item % C::UNITS]);
+                    const int ab = item % C::UNITS;
+                    if (item >= C::UNITS) ok = wait(&a_empty[ab], (uint32_t)(item / C::UNITS - 1) & 1u);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx_elect(a_bar + ab * 8, C::A_BYTES);
+                    const int a_row = (DKV ? w.k_first : w.q_first) + w.a_first, a_heads = DKV ? p.kv_heads : p.heads;
+                    load_head<C::BLOCKS>(&p.tmA[0], base + ab * C::A_BYTES, C::A_BLOCK, a_heads, w.head, a_row, a_bar + ab * 8);
+                    load_head<C::BLOCKS>(&p.tmA[1], base + ab * C::A_BYTES + C::A_TILE, C::A_BLOCK, a_heads, w.head, a_row, a_bar + ab * 8);
+                    ++item;
                 }
-                t -= w.tiles;
-                more = ok && take(index++);
-                if (!more) w.tiles = 0;
-                item += w.tiles > 0;
-                in_head = t;
+                int h = w.h0, t = 0;
+                for (int j = 0; j < w.tiles && ok; ++j) {
+                    if (round > 0) ok = wait(&empty[st], (round - 1) & 1u);
+                    if (!ok) break;
+                    const uint32_t b = bar + st * 8, dst = base + C::RING + st * C::STAGE;
+                    mbar_arrive_expect_tx_elect(b, C::STAGE);
+                    const int row = (DKV ? w.q_first : w.k_first) + w.first + t * kTile;
+                    load_head<C::BLOCKS>(&p.tm[0], dst, C::BLOCK, DKV ? p.heads : p.kv_heads, DKV ? h : w.kvh, row, b);
+                    load_head<C::BLOCKS>(&p.tm[1], dst + C::TILE, C::BLOCK, DKV ? p.heads : p.kv_heads, DKV ? h : w.kvh, row, b);
+                    if (++t == w.tiles_per_head) {
+                        t = 0;
+                        ++h;
+                    }
+                    if (++st == C::STAGES) {
+                        st = 0;
+                        ++round;
+                    }
+                }
+                if (ok) next();
             }
-            return more;
-        };
-        // S or dP of the tile that the walk is at
-        auto scores = [&](int which) {
-            const int ab = item % C::UNITS;
-            if (which == 0) {
-                standing();
-                need(&full[st], parity, DEV_ERR_FULL_WAIT);
-                while (in_head >= w.tiles_per_head) in_head -= w.tiles_per_head;
-                const int valid = (DKV ? w.q_len : w.k_len) - w.first - in_head * kTile;
-                if (ok && valid < kTile) zero_rows(smem + C::RING + st * C::STAGE, C::BLOCK, 2 * C::BLOCKS, valid, kTile);
+        } else if (warp <= NG) {
+            // ---- products of one group
+            const int g = warp - 1, before = g == 0 ? NG - 1 : g - 1;
+            constexpr uint32_t idesc_s = umma_idesc_bf16(kStand, kTile), idesc_acc = umma_idesc_bf16(kStand, HD) | (1u << 16);  // streamed tile: its K extent in rows
+            const uint32_t base = smem_u32(smem), buf = tmem + g * 2 * kTile;
+            const uint64_t a_d = umma_desc_k128(base), k_d = umma_desc_k128(base + C::RING), n_d = umma_desc_n128(base + C::RING, C::BLOCK);
+            auto wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, code)); };
+            auto product = [&](uint32_t d, int which, int ab, int st) {
+                const uint64_t a = a_d + (uint64_t)(uint32_t)((ab * C::A_BYTES + which * C::A_TILE) >> 4), b = k_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4);
+#pragma unroll
+                for (int i = 0; i < C::BLOCKS; ++i) umma_bf16_x4<2, 2>(d, a + i * (C::A_BLOCK >> 4), b + i * (C::BLOCK >> 4), idesc_s, i > 0);
+            };
+            auto accumulate = [&](uint32_t d, uint32_t a, int which, int st, bool more) {
+                static_assert(kTile == 64, "four products of 16 rows");
+                umma_bf16_ts_x4<8, 128>(d, a, n_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4), idesc_acc, more);
+            };
+            bool ok = true;
+            auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
+            // Two of them. A look at a barrier costs 90 cycles even if it is ready, so both at once where that is likely; beside three groups the
+            // looks in vain cost more than they save (8 x 4 096, 64 columns: 1 200 us, else 1 100; 1 x 8 192, 128 columns: 1 730, else 1 790).
+            auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+                if (HD == 64 || !__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
+                    need(a, pa, DEV_ERR_ACC_WAIT);
+                    need(b, pb, DEV_ERR_ACC_WAIT);
+                }
+            };
+            auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)); };
+            // The walk over this group's tiles, which S and dP are at.
+            int index = 0, item = -1, seen = -1;  // units taken; units with tiles, less one; the last of those whose standing rows are known to be there
+            int t = g, in_head = g, st = g;       // the tile in its unit, in its head; its stage. The first tile of this group is tile g of all.
+            uint32_t parity = 0;                  // of the stage
+            bool more = true;
+            w.tiles = 0;
+            auto standing = [&]() {
+                if (seen != item) need(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u, DEV_ERR_FULL_WAIT);
+                seen = item;
+            };
+            // To the next tile, not past `units` more units: a later one waits for results that this warp may owe products to. False if that is too
+            // far, or there is no more. A unit's standing rows are left behind: every group sees that they were there, also where it has no tile of the unit, since
+            // a barrier's parity tells only the next phase from the last one.
+            auto find = [&](int units) {
+                while (more && t >= w.tiles) {
+                    if (units == 0) return false;
+                    --units;
+                    if (w.tiles > 0) {
+                        standing();
+                        umma_commit_elect(&a_empty[item % C::UNITS]);
+                    }
+                    t -= w.tiles;
+                    more = ok && take(index++);
+                    if (!more) w.tiles = 0;
+                    item += w.tiles > 0;
+                    in_head = t;
+                }
+                return more;
+            };
+            // S or dP of the tile that the walk is at
+            auto scores = [&](int which) {
+                const int ab = item % C::UNITS;
+                if (which == 0) {
+                    standing();
+                    need(&full[st], parity, DEV_ERR_FULL_WAIT);
+                    while (in_head >= w.tiles_per_head) in_head -= w.tiles_per_head;
+                    const int valid = (DKV ? w.q_len : w.k_len) - w.first - in_head * kTile;
+                    if (ok && valid < kTile) zero_rows(smem + C::RING + st * C::STAGE, C::BLOCK, 2 * C::BLOCKS, valid, kTile);
+                    tc_fence_after();
+                }
+                if (!ok) return;
+                product(buf + which * kTile, which, ab, st);
+                umma_commit_elect(which ? &dp_full[g] : &s_full[g]);
+            };
+            bool have = false, early = false;
+            for (uint32_t mine = 0;; ++mine) {
+                if (!have && more) have = find(INT32_MAX);
+                if (!ok || !have) break;
+                if (!early) scores(0);
+                scores(1);
+                const int at = st, unit = item;
+                const bool first = t == 0, last = t == w.tiles - 1, follows = g > 0 || mine > 0;
+                const uint32_t turns = (g > 0 ? mine : mine - 1) & 1u;  // of the group whose tile is before this one
+                t += NG;
+                in_head += NG;
+                st += NG;
+                if (st >= C::STAGES) {
+                    st -= C::STAGES;
+                    parity ^= 1u;
+                }
+                // M += P K or dV += P^T dO, behind the tile before; then S of the next tile in P's place while the group is at dS
+                if (follows)
+                    need_both(&p_full[g], mine & 1u, &p_added[before], turns);
+                else
+                    need(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
+                // the results of the unit before have left the accumulators (behind the tile before, which has seen those of the unit before that leave)
+                if (first && unit > 0) need(acc_free, (uint32_t)(unit - 1) & 1u, DEV_ERR_ACC_WAIT);
+                if (!ok) break;
                 tc_fence_after();
+                accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
+                umma_commit_elect(&p_added[g]);
+                have = find(1);
+                // 64 columns: six stages, the tile is as good as there; 128: four, dS comes first where it is not
+                early = have && ((HD == 64 && seen == item) || (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity));
+                if (early) scores(0);
+                if (follows)
+                    need_both(&ds_full[g], mine & 1u, &ds_added[before], turns);
+                else
+                    need(&ds_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
+                if (!ok) break;
+                tc_fence_after();
+                accumulate(tmem + C::ACC + HD, buf + kTile, 0, at, !first);
+                umma_commit_elect(&ds_added[g]);
+                umma_commit_elect(&empty[at]);
+                if (last) umma_commit_elect(acc_done);
             }
-            if (!ok) return;
-            product(buf + which * kTile, which, ab, st);
-            umma_commit_elect(which ? &dp_full[g] : &s_full[g]);
-        };
-        bool have = find(INT32_MAX);
-        if (have) {
-            scores(0);
-            scores(1);
         }
-        for (uint32_t mine = 0; ok && have; ++mine) {
-            const int at = st, unit = item;
-            const bool first = t == 0, last = t == w.tiles - 1, follows = g > 0 || mine > 0;
-            const uint32_t turns = (g > 0 ? mine : mine - 1) & 1u;  // of the group whose tile is before this one
-            t += NG;
-            in_head += NG;
-            st += NG;
-            if (st >= C::STAGES) {
-                st -= C::STAGES;
-                parity ^= 1u;
-            }
-            // M += P K or dV += P^T dO, behind the tile before; then S of the next tile in P's place while the group is at dS
-            if (follows)
-                need_both(&p_full[g], mine & 1u, &p_added[before], turns);
-            else
-                need(&p_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
-            // the results of the unit before have left the accumulators (behind the tile before, which has seen those of the unit before that leave)
-            if (first && unit > 0) need(acc_free, (uint32_t)(unit - 1) & 1u, DEV_ERR_ACC_WAIT);
-            if (!ok) break;
-            tc_fence_after();
-            accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
-            umma_commit_elect(&p_added[g]);
-            have = find(1);
-            // 64 columns: six stages, the tile is as good as there; 128: four, dS comes first where it is not
-            const bool early = have && ((HD == 64 && seen == item) || (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity));
-            if (early) scores(0);
-            if (follows)
-                need_both(&ds_full[g], mine & 1u, &ds_added[before], turns);
-            else
-                need(&ds_full[g], mine & 1u, DEV_ERR_ACC_WAIT);
-            if (!ok) break;
-            tc_fence_after();
-            accumulate(tmem + C::ACC + HD, buf + kTile, 0, at, !first);
-            umma_commit_elect(&ds_added[g]);
-            umma_commit_elect(&empty[at]);
-            if (last) umma_commit_elect(acc_done);
-            if (!have && more) have = find(INT32_MAX);
-            if (have && !early) scores(0);
-            if (have) scores(1);
-        }
-    } else if (warp >= 4) {
+    } else if (warp < 4 + 4 * NG) {
         // ---- P and dS
+        if (HD == 64) reg_inc<120>();
         const int group = (warp >> 2) - 1, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, buf = tmem + lanes + group * 2 * kTile;
         float* const stats = (float*)(smem + C::ROWS) + group * 4 * kTile;  // -lse and -D of streamed queries, twice
-        float* const sums = (float*)(smem + C::ROWS);                       // or the groups' row sums
         bool ok = true;
         // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, p.status, DEV_ERR_ACC_WAIT));
+            if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
             tc_fence_after();
         };
         int item = 0, turn = 0;  // units with tiles so far; tiles of all units before, modulo the groups
@@ -386,37 +401,45 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 }
                 wait(&s_full[group], ph);
                 F2 pr[kTile / 2];
-                auto weights = [&](auto masked) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t s[2][16], v[16];
-                        tmem_ld16(buf + half * 32, s[0]);
-                        tmem_ld16(buf + half * 32 + 16, s[1]);
+                if (!whole) {
+#pragma unroll 1
+                    for (int c = 0; c < kTile; c += 16) {
+                        const int from = min(max(c_lo - c, 0), 16), to = min(max(c_hi - c, 0), 16);
+                        if (__all_sync(0xffffffffu, from == 0 && to == 16)) continue;
+                        const uint32_t seen = (1u << to) - 1u & ~((1u << from) - 1u);
+                        uint32_t s[16];
+                        tmem_ld16(buf + c, s);
                         tc_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            float4 l4 = make_float4(nl, nl, nl, nl);
-                            if constexpr (DKV) l4 = *(const float4*)(q_stats + half * 32 + i);
-#pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                const int c = half * 32 + i + e, k = i + e;
-                                float x, y;
-                                split2(fma2(f2(__uint_as_float(s[k >> 4][k & 15]), __uint_as_float(s[k >> 4][(k & 15) + 1])), scale2, e ? f2(l4.z, l4.w) : f2(l4.x, l4.y)), x, y);
-                                x = exp2_fast(x);
-                                y = exp2_fast(y);
-                                if (masked.value && (c < c_lo || c >= c_hi)) x = 0.f;
-                                if (masked.value && (c + 1 < c_lo || c + 1 >= c_hi)) y = 0.f;
-                                pr[c >> 1] = f2(x, y);
-                                v[k >> 1] = pack2(x, y);
-                            }
-                        }
-                        tmem_st16(buf + half * 16, v);
+                        for (int i = 0; i < 16; ++i)
+                            if (!(seen & 1u << i)) s[i] = 0xff800000u;
+                        tmem_st16(buf + c, s);
                     }
-                };
-                if (whole)
-                    weights(std::false_type());
-                else
-                    weights(std::true_type());
+                    tc_wait_st();
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t s[2][16], v[16];
+                    tmem_ld16(buf + half * 32, s[0]);
+                    tmem_ld16(buf + half * 32 + 16, s[1]);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        float4 l4 = make_float4(nl, nl, nl, nl);
+                        if constexpr (DKV) l4 = *(const float4*)(q_stats + half * 32 + i);
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const int k = i + e;
+                            float x, y;
+                            split2(fma2(f2(__uint_as_float(s[k >> 4][k & 15]), __uint_as_float(s[k >> 4][(k & 15) + 1])), scale2, e ? f2(l4.z, l4.w) : f2(l4.x, l4.y)), x, y);
+                            x = exp2_fast(x);
+                            y = exp2_fast(y);
+                            pr[(half * 32 + k) >> 1] = f2(x, y);
+                            v[k >> 1] = pack2(x, y);
+                        }
+                    }
+                    tmem_st16(buf + half * 16, v);
+                }
                 tc_wait_st();
                 tc_fence_before();
                 mbar_arrive(&p_full[group]);
@@ -455,89 +478,118 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 mbar_arrive(&ds_full[group]);
             }
             turn = (turn + w.tiles) % NG;
-            // ---- results of the unit
-            const bool any = w.tiles > 0;
-            if (any) wait(acc_done, (uint32_t)item & 1u);
-            if constexpr (!DKV) {
-                if (any) {
-                    sums[group * kStand + r] = sum;
-                    named_barrier(1 + NG, NG * 128);
-                    sum = 0.f;
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) sum += sums[g * kStand + r];
-                    if (group == 0 && live) p.d[(int64_t)w.head * p.rows_q + grow] = sum - nd;
-                }
-            }
-            // 64 bytes of a row at a time, dealt to the groups: 32 columns, or 16 of an fp32 sum
-            uint8_t* const out = smem + C::OUT + (warp - 4) * 2048;
-            const int warp_row = (warp & 3) * 32, rows = w.a_rows - warp_row, grow0 = grow - (r & 31);
-            bool freed = false;
-            auto free_sums = [&]() {  // this warp's last look at the accumulators
-                tc_fence_before();
+            if (!DKV && w.tiles > 0) {
+                const int at = item & 1;
+                if (item >= 2) wait(&sum_empty[at], (uint32_t)(item / 2 - 1) & 1u);
+                ((float*)(smem + C::ROWS))[(at * NG + group) * kStand + r] = sum;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_free);
-                freed = true;
-            };
-            auto store = [&](auto wide) {
-                constexpr int COLS = wide.value ? 16 : 32, PIECES = (DKV ? 2 : 1) * HD / COLS;
-#pragma unroll 1
-                for (int k = group; k < PIECES; k += NG) {
-                    const bool second = DKV && k >= HD / COLS;  // dV
-                    const int c = (k % (HD / COLS)) * COLS;
-                    const float f = second ? 1.f : p.scale;
-                    float v[COLS];
-                    uint32_t a[COLS / 16][16];
-#pragma unroll
-                    for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + (second ? 0 : HD) + c + 16 * i, a[i]);
-                    if constexpr (!DKV) {
-                        uint32_t m[COLS / 16][16];
-#pragma unroll
-                        for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + c + 16 * i, m[i]);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < COLS; ++i) v[i] = f * fmaf(-sum, __uint_as_float(m[i >> 4][i & 15]), __uint_as_float(a[i >> 4][i & 15]));
-                    } else {
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < COLS; ++i) v[i] = f * __uint_as_float(a[i >> 4][i & 15]);
-                    }
-                    if (k + NG >= PIECES) free_sums();
-                    uint4 x[4];
-                    char* to;
-                    int64_t stride;
-                    if constexpr (wide.value) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
-                        stride = (int64_t)p.kv_heads * p.hd * 4;
-                        to = (char*)p.partial + (((int64_t)(second ? p.parts : 0) + w.part) * p.rows_k + grow0) * stride + ((int64_t)w.kvh * p.hd + c) * 4;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]), pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
-                        stride = (second ? p.out1_stride : p.out0_stride) * 2;
-                        to = (char*)(second ? p.out1 : p.out0) + grow0 * stride + ((int64_t)w.head * p.hd + c) * 2;
-                    }
-                    store_rows(out, x, to, stride, rows, (p.hd - c) * (wide.value ? 4 : 2) / 16);
-                }
-            };
-            if (any) {
-                if (DKV && p.partial)
-                    store(std::true_type());
-                else
-                    store(std::false_type());
-                if (!freed) free_sums();
-                ++item;
-            } else if (live) {  // nothing is seen: zeros
-                for (int k = group; k < (DKV ? 2 : 1) * p.hd / 8; k += NG) {
-                    const bool second = k >= p.hd / 8;
-                    const int c = (second ? k - p.hd / 8 : k) * 8;
-                    if (DKV && p.partial) {
-                        float* const to = p.partial + ((((int64_t)(second ? p.parts : 0) + w.part) * p.rows_k + grow) * p.kv_heads + w.kvh) * p.hd + c;
-                        *(uint4*)to = *(uint4*)(to + 4) = make_uint4(0u, 0u, 0u, 0u);
-                    } else {
-                        *(uint4*)((second ? p.out1 + grow * p.out1_stride : p.out0 + grow * p.out0_stride) + (int64_t)w.head * p.hd + c) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                }
+                if (lane == 0) mbar_arrive(&sum_full[at]);
             }
+            item += w.tiles > 0;
+        }
+    } else {
+        // ---- results
+        if (HD == 64) reg_dec<72>();
+        const int r = tid & 127, warp_row = (warp & 3) * 32;
+        const uint32_t lanes = (uint32_t)warp_row << 16;
+        uint8_t* const out = smem + C::OUT + (warp & 3) * 2048;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+            if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
+            tc_fence_after();
+        };
+        int item = 0;
+        for (int index = 0; take(index); ++index) {
+            const bool live = r < w.a_rows;
+            const int rows = w.a_rows - warp_row, grow = (DKV ? w.k_first : w.q_first) + w.a_first + r, grow0 = grow - lane;  // rows of the buffers
+            if (w.tiles == 0) {  // nothing is seen: zeros
+                if (live)
+                    for (int k = 0; k < (DKV ? 2 : 1) * p.hd / 8; ++k) {
+                        const bool second = k >= p.hd / 8;
+                        const int c = (second ? k - p.hd / 8 : k) * 8;
+                        if (DKV && p.partial) {
+                            float* const to = p.partial + ((((int64_t)(second ? p.parts : 0) + w.part) * p.rows_k + grow) * p.kv_heads + w.kvh) * p.hd + c;
+                            *(uint4*)to = *(uint4*)(to + 4) = make_uint4(0u, 0u, 0u, 0u);
+                        } else {
+                            *(uint4*)((second ? p.out1 + grow * p.out1_stride : p.out0 + grow * p.out0_stride) + (int64_t)w.head * p.hd + c) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                    }
+                continue;
+            }
+            float sum = 0.f, d = 0.f;
+            float* const d_at = p.d + (int64_t)w.head * p.rows_q + grow;
+            if (!DKV && live) d = __ldcg(d_at);
+            wait(acc_done, (uint32_t)item & 1u);
+            if constexpr (!DKV) {
+                const int at = item & 1;
+                wait(&sum_full[at], (uint32_t)(item / 2) & 1u);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) sum += ((const float*)(smem + C::ROWS))[(at * NG + g) * kStand + r];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sum_empty[at]);
+                if (live) *d_at = d + sum;
+            }
+            ++item;
+            // 64 bytes of a row are a piece, 32 columns or 16 of an fp32 sum; so few at once to keep the code short
+            auto store = [&](auto wide) {
+                constexpr int COLS = wide.value ? 16 : 32, PER = HD / COLS, PIECES = (DKV ? 2 : 1) * PER, AT_ONCE = 1;
+#pragma unroll 1
+                for (int k0 = 0; k0 < PIECES; k0 += AT_ONCE) {
+                    uint4 x[AT_ONCE][4];
+#pragma unroll
+                    for (int j = 0; j < AT_ONCE; ++j) {
+                        const bool sec = DKV && k0 + j >= PER;  // dV
+                        const int c = (k0 + j - (sec ? PER : 0)) * COLS;
+                        const float f = sec ? 1.f : p.scale;
+                        float v[COLS];
+                        uint32_t a[COLS / 16][16];
+#pragma unroll
+                        for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + (sec ? 0 : HD) + c + 16 * i, a[i]);
+                        if constexpr (!DKV) {
+                            uint32_t m[COLS / 16][16];
+#pragma unroll
+                            for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + c + 16 * i, m[i]);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i) v[i] = f * fmaf(-sum, __uint_as_float(m[i >> 4][i & 15]), __uint_as_float(a[i >> 4][i & 15]));
+                        } else {
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < COLS; ++i) v[i] = f * __uint_as_float(a[i >> 4][i & 15]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if constexpr (wide.value)
+                                x[j][i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                            else
+                                x[j][i] = make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]), pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
+                    }
+                    if (k0 + AT_ONCE >= PIECES) {  // the last look at the accumulators
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acc_free);
+                    }
+#pragma unroll
+                    for (int j = 0; j < AT_ONCE; ++j) {
+                        const bool sec = DKV && k0 + j >= PER;
+                        const int c = (k0 + j - (sec ? PER : 0)) * COLS;
+                        char* to;
+                        int64_t stride;
+                        if constexpr (wide.value) {
+                            stride = (int64_t)p.kv_heads * p.hd * 4;
+                            to = (char*)p.partial + (((int64_t)(sec ? p.parts : 0) + w.part) * p.rows_k + grow0) * stride + ((int64_t)w.kvh * p.hd + c) * 4;
+                        } else {
+                            stride = (sec ? p.out1_stride : p.out0_stride) * 2;
+                            to = (char*)(sec ? p.out1 : p.out0) + grow0 * stride + ((int64_t)w.head * p.hd + c) * 2;
+                        }
+                        store_rows(out, x[j], to, stride, rows, (p.hd - c) * (wide.value ? 4 : 2) / 16);
+                    }
+                }
+            };
+            if (DKV && p.partial)
+                store(std::true_type());
+            else
+                store(std::false_type());
         }
     }
     tc_fence_before();
