@@ -120,12 +120,12 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         fence_mbar_init();
     }
     // The first warp works out the units. Its first one does not need the barriers.
-    int cursor = blockIdx.x;
+    AttnWalk walk;
     Units<NG> w;
     auto next_units = [&]() {
         AttnUnit u;
         w.tiles = -1;
-        if (next_unit<false>(p, cursor, u, [&](int len) { return p.by_parts.div((len + kStand - 1) / kStand * p.group + p.parts - 1); })) units_of<NG>(p, u, w);
+        if (next_unit<false>(p, walk, u, [&](int len) { return p.by_parts.div((len + kStand - 1) / kStand * p.group + p.parts - 1); })) units_of<NG>(p, u, w);
     };
     if (warp == 0) {
         if (lane == 0) {
@@ -482,17 +482,18 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     using C = Cfg<HD>;
     const int G = c.heads / c.kv_heads;
     const int64_t blocks = (c.max_q + kStand - 1) / kStand, all = blocks * c.n_seqs * c.heads;
-    // Units to themselves where every group of every SM gets two, us (one unit at a time against units of their own): 8 ragged x 2 048, 12 heads of 128
-    // 88 against 77; 32 ragged x 512, 14 heads of 64 49 against 41; 1 x 4 096 of them 84 against 88; 1 x 1 000 17 against 37.
-    p.parts = all <= 2 * C::GROUPS * num_sms ? 1 : C::GROUPS;
+    // Units to themselves where every group of every SM gets four, us (one unit at a time against units of their own): 1 x 8 192, 28 heads of 128
+    // 467 against 411; 8 x 4 096, 14 heads of 64 390 against 319; 32 ragged x 512 of them 41 against 34; 3 x 2 777 of them in chunks of 1 024 44
+    // against 75; 1 x 1 000 of them 16 against 37.
+    p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;
     const int64_t units = (blocks * G + p.parts - 1) / p.parts * c.n_seqs * c.kv_heads;
     if (units >= 1 << 30 || blocks * G >= 1 << 30) return (int)cudaErrorInvalidValue;
-    p.units = (int)units;
+    order_units(p, c, false, (blocks * G + p.parts - 1) / p.parts, (int64_t)c.chunk / kStand * G / p.parts);
     p.by_fast = FastDiv::of(c.kv_heads);
     p.by_parts = FastDiv::of(p.parts);
     const cudaError_t e = allow_shared<k_attn_fwd<HD>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_k(k_attn_fwd<HD>, dim3((unsigned)(p.units < num_sms ? p.units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, false, p);
+    return (int)launch_k(k_attn_fwd<HD>, dim3((unsigned)(units < num_sms ? units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, false, p);
 }
 
 }  // namespace
@@ -511,9 +512,8 @@ AttnDev attn_dev(const AttnCall& c) {
     p.kv_heads = c.kv_heads;
     p.group = c.heads / c.kv_heads;
     p.by_group = FastDiv::of(p.group);
-    p.by_seqs = FastDiv::of(c.n_seqs);
     p.by_chunk = FastDiv::of(c.chunk > 0 ? c.chunk : 1);
-    p.by_fast = p.by_parts = FastDiv::of(1);
+    p.by_fast = p.by_parts = p.by_turns = FastDiv::of(1);
     p.hd = c.hd;
     p.causal = c.causal;
     p.chunk = c.chunk;
@@ -523,6 +523,16 @@ AttnDev attn_dev(const AttnCall& c) {
     p.lse = c.lse;
     p.status = c.status;
     return p;
+}
+
+// slots: of the longest sequence; chunk_slots: of a chunk. Queries may begin in the middle of a chunk, so that they touch one more.
+void order_units(AttnDev& p, const AttnCall& c, bool keys, int64_t slots, int64_t chunk_slots) {
+    const int64_t period = c.chunk > 0 && chunk_slots < 1 ? 1 : chunk_slots;
+    p.by_chunk_order = c.chunk > 0 && period < slots;
+    p.period = (int)(p.by_chunk_order ? period : slots);
+    const int64_t turns = !p.by_chunk_order ? 1 : keys ? (slots + period - 1) / period : (slots + 2 * period - 1) / period;
+    p.by_turns = FastDiv::of(turns);
+    p.levels = (int)(turns * p.period);
 }
 
 bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box) {

@@ -25,6 +25,7 @@
 // is what such a call waits for (32 sequences of up to 512 queries, 14 / 2 heads of 64 columns: 112 us; with a mask variant of P and
 // unrolled waits 157 us; then with the results in the groups' hands 152 us).
 #include "train_attn.cuh"
+#include <algorithm>
 #include <cstring>
 #include <type_traits>
 
@@ -138,12 +139,12 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         fence_mbar_init();
     }
     // The first warp works out the units. Its first one does not need the barriers.
-    int cursor = blockIdx.x;
+    AttnWalk walk;
     Unit w;
     auto next = [&]() {
         AttnUnit u;
         w.tiles = -1;
-        if (next_unit<DKV>(p, cursor, u, [](int len) { return (len + kStand - 1) / kStand; })) unit_of<DKV>(p, u, w);
+        if (next_unit<DKV>(p, walk, u, [](int len) { return (len + kStand - 1) / kStand; })) unit_of<DKV>(p, u, w);
     };
     if (warp == 0) {
         if (lane == 0) {
@@ -244,15 +245,14 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             };
             bool ok = true;
             auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
-            // Two of them. A look at a barrier costs 90 cycles even if it is ready, so both at once where that is likely; beside three groups the
-            // looks in vain cost more than they save (8 x 4 096, 64 columns: 1 200 us, else 1 100; 1 x 8 192, 128 columns: 1 730, else 1 790).
-            auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
-                if (HD == 64 || !__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
-                    need(a, pa, DEV_ERR_ACC_WAIT);
-                    need(b, pb, DEV_ERR_ACC_WAIT);
-                }
-            };
-            auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)); };
+            // Two of them, both at once where that is likely: a look at a barrier costs 90 cycles even if it is ready.
+        auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+            if (!__all_sync(0xffffffffu, mbar_test_wait(a, pa) & mbar_test_wait(b, pb))) {
+                need(a, pa, DEV_ERR_ACC_WAIT);
+                need(b, pb, DEV_ERR_ACC_WAIT);
+            }
+        };
+        auto there = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar, parity)); };
             // The walk over this group's tiles, which S and dP are at.
             int index = 0, item = -1, seen = -1;  // units taken; units with tiles, less one; the last of those whose standing rows are known to be there
             int t = g, in_head = g, st = g;       // the tile in its unit, in its head; its stage. The first tile of this group is tile g of all.
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 umma_commit_elect(&p_added[g]);
                 have = find(1);
                 // 64 columns: six stages, the tile is as good as there; 128: four, dS comes first where it is not
-                early = have && ((HD == 64 && seen == item) || (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity));
+                early = have && (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity);
                 if (early) scores(0);
                 if (follows)
                     need_both(&ds_full[g], mine & 1u, &ds_added[before], turns);
@@ -530,60 +530,50 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 if (live) *d_at = d + sum;
             }
             ++item;
-            // 64 bytes of a row are a piece, 32 columns or 16 of an fp32 sum; so few at once to keep the code short
+            // 64 bytes of a row at a time, 32 columns or 16 of an fp32 sum
             auto store = [&](auto wide) {
-                constexpr int COLS = wide.value ? 16 : 32, PER = HD / COLS, PIECES = (DKV ? 2 : 1) * PER, AT_ONCE = 1;
+                constexpr int COLS = wide.value ? 16 : 32, PER = HD / COLS, PIECES = (DKV ? 2 : 1) * PER;
 #pragma unroll 1
-                for (int k0 = 0; k0 < PIECES; k0 += AT_ONCE) {
-                    uint4 x[AT_ONCE][4];
+                for (int k = 0; k < PIECES; ++k) {
+                    const bool second = DKV && k >= PER;  // dV
+                    const int c = (k - (second ? PER : 0)) * COLS;
+                    const float f = second ? 1.f : p.scale;
+                    float v[COLS];
+                    uint32_t a[COLS / 16][16];
 #pragma unroll
-                    for (int j = 0; j < AT_ONCE; ++j) {
-                        const bool sec = DKV && k0 + j >= PER;  // dV
-                        const int c = (k0 + j - (sec ? PER : 0)) * COLS;
-                        const float f = sec ? 1.f : p.scale;
-                        float v[COLS];
-                        uint32_t a[COLS / 16][16];
+                    for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + (second ? 0 : HD) + c + 16 * i, a[i]);
+                    if constexpr (!DKV) {
+                        uint32_t m[COLS / 16][16];
 #pragma unroll
-                        for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + (sec ? 0 : HD) + c + 16 * i, a[i]);
-                        if constexpr (!DKV) {
-                            uint32_t m[COLS / 16][16];
+                        for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + c + 16 * i, m[i]);
+                        tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < COLS / 16; ++i) tmem_ld16(tmem + lanes + C::ACC + c + 16 * i, m[i]);
-                            tc_wait_ld();
+                        for (int i = 0; i < COLS; ++i) v[i] = f * fmaf(-sum, __uint_as_float(m[i >> 4][i & 15]), __uint_as_float(a[i >> 4][i & 15]));
+                    } else {
+                        tc_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < COLS; ++i) v[i] = f * fmaf(-sum, __uint_as_float(m[i >> 4][i & 15]), __uint_as_float(a[i >> 4][i & 15]));
-                        } else {
-                            tc_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < COLS; ++i) v[i] = f * __uint_as_float(a[i >> 4][i & 15]);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if constexpr (wide.value)
-                                x[j][i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
-                            else
-                                x[j][i] = make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]), pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
+                        for (int i = 0; i < COLS; ++i) v[i] = f * __uint_as_float(a[i >> 4][i & 15]);
                     }
-                    if (k0 + AT_ONCE >= PIECES) {  // the last look at the accumulators
+                    if (k == PIECES - 1) {  // the last look at the accumulators
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(acc_free);
                     }
+                    uint4 x[4];
+                    char* to;
+                    int64_t stride;
+                    if constexpr (wide.value) {
 #pragma unroll
-                    for (int j = 0; j < AT_ONCE; ++j) {
-                        const bool sec = DKV && k0 + j >= PER;
-                        const int c = (k0 + j - (sec ? PER : 0)) * COLS;
-                        char* to;
-                        int64_t stride;
-                        if constexpr (wide.value) {
-                            stride = (int64_t)p.kv_heads * p.hd * 4;
-                            to = (char*)p.partial + (((int64_t)(sec ? p.parts : 0) + w.part) * p.rows_k + grow0) * stride + ((int64_t)w.kvh * p.hd + c) * 4;
-                        } else {
-                            stride = (sec ? p.out1_stride : p.out0_stride) * 2;
-                            to = (char*)(sec ? p.out1 : p.out0) + grow0 * stride + ((int64_t)w.head * p.hd + c) * 2;
-                        }
-                        store_rows(out, x[j], to, stride, rows, (p.hd - c) * (wide.value ? 4 : 2) / 16);
+                        for (int i = 0; i < 4; ++i) x[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+                        stride = (int64_t)p.kv_heads * p.hd * 4;
+                        to = (char*)p.partial + (((int64_t)(second ? p.parts : 0) + w.part) * p.rows_k + grow0) * stride + ((int64_t)w.kvh * p.hd + c) * 4;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = make_uint4(pack2(v[8 * i], v[8 * i + 1]), pack2(v[8 * i + 2], v[8 * i + 3]), pack2(v[8 * i + 4], v[8 * i + 5]), pack2(v[8 * i + 6], v[8 * i + 7]));
+                        stride = (second ? p.out1_stride : p.out0_stride) * 2;
+                        to = (char*)(second ? p.out1 : p.out0) + grow0 * stride + ((int64_t)w.head * p.hd + c) * 2;
                     }
+                    store_rows(out, x, to, stride, rows, (p.hd - c) * (wide.value ? 4 : 2) / 16);
                 }
             };
             if (DKV && p.partial)
@@ -632,45 +622,52 @@ __global__ void __launch_bounds__(256) k_attn_dot(const bf16* __restrict__ d_out
     }
 }
 
-// dK and dV from the parts of the query heads, added in their order
+// dK and dV from the parts of the query heads, added in their order; kJoinRows rows a block
+constexpr int kJoinRows = 8;
 __global__ void __launch_bounds__(256) k_attn_join(const float* __restrict__ partial, int parts, const int* cu_k, int n_seqs, int64_t rows, int kv_heads, int hd, bf16* dk,
                                                    int64_t dk_stride, bf16* dv, int64_t dv_stride) {
-    pdl_wait();
     const int per_row = kv_heads * hd / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / per_row;
-    if (row >= rows || row < cu_k[0] || row >= cu_k[n_seqs]) return;
-    const int c = (int)(i % per_row) * 4;
     const int64_t plane = rows * kv_heads * hd;
-    const float* src = partial + (int64_t)blockIdx.y * parts * plane + row * kv_heads * hd + c;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < parts; ++q) {
-        const float4 v = __ldcg((const float4*)(src + q * plane));
-        a.x += v.x;
-        a.y += v.y;
-        a.z += v.z;
-        a.w += v.w;
+    const float* src = partial + (int64_t)blockIdx.y * parts * plane;
+    pdl_wait();
+    const int begin = cu_k[0], end = cu_k[n_seqs];
+    for (int i = threadIdx.x; i < kJoinRows * per_row; i += 256) {
+        const int r = i / per_row, c = (i - r * per_row) * 4;
+        const int64_t row = (int64_t)blockIdx.x * kJoinRows + r;
+        if (row >= rows || row < begin || row >= end) continue;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int q = 0; q < parts; ++q) {
+            const float4 v = __ldcg((const float4*)(src + q * plane + row * kv_heads * hd + c));
+            a.x += v.x;
+            a.y += v.y;
+            a.z += v.z;
+            a.w += v.w;
+        }
+        bf16* dst = blockIdx.y ? dv + row * dv_stride : dk + row * dk_stride;
+        *(uint2*)(dst + c) = make_uint2(pack2(a.x, a.y), pack2(a.z, a.w));
     }
-    bf16* dst = blockIdx.y ? dv + row * dv_stride : dk + row * dk_stride;
-    *(uint2*)(dst + c) = make_uint2(pack2(a.x, a.y), pack2(a.z, a.w));
 }
 
 template <int HD, bool DKV>
-int run(const AttnDev& p, int num_sms, cudaStream_t s, bool pdl) {
+int run(const AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) {
     using C = Cfg<HD>;
     const cudaError_t e = allow_shared<k_attn_bwd<HD, DKV>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3((unsigned)(p.units < num_sms ? p.units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
+    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3((unsigned)(units < num_sms ? units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
 }
 
 int64_t units_for(const AttnCall& c, int most, int fast) { return (int64_t)((most + kStand - 1) / kStand) * c.n_seqs * fast; }
 
-// Blocks of dK, dV by query heads: one block adds all heads of its kv head up where that gives each of the 148 SMs two units of work to even
-// out unequal lengths; else the heads are dealt to as many units as that takes, and their sums are joined through the workspace.
+// Parts of the query heads of a kv head for dK, dV. One block adds all of them up where there are one and a half units of work for each of the
+// 148 SMs, as the packed rows let expect; else the heads are dealt to as many units as that takes, and their sums are joined through the workspace.
+// All heads together against this, us, whole call: 1 x 4 096, 14 / 2 heads of 64 296 against 134; 8 ragged x 2 048, 12 / 2 of 128 228 against 175.
+// Parts of single heads against this: 8 x 4 096, 14 / 2 of 64 986 against 852; 1 x 8 192, 28 / 4 of 128 1 415 against 1 363.
 int parts_of(const AttnCall& c) {
     const int G = c.heads / c.kv_heads;
-    const int64_t units = units_for(c, c.max_k, c.kv_heads);
+    const int64_t most = units_for(c, c.max_k, c.kv_heads), expected = (c.rows_k / kStand + c.n_seqs / 2) * c.kv_heads, units = std::max<int64_t>(std::min(most, expected), 1);
     int parts = 1;
-    while (parts < G && units * parts < 2 * 148) ++parts;
+    while (parts < G && units * parts < 148 * 3 / 2) ++parts;
     const int per = (G + parts - 1) / parts;
     return (G + per - 1) / per;
 }
@@ -709,7 +706,7 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         if (rc) return rc;
         const int64_t units = units_for(c, c.max_q, c.heads);
         if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
-        p.units = (int)units;
+        order_units(p, c, false, (c.max_q + kStand - 1) / kStand, c.chunk / kStand);
         p.by_fast = FastDiv::of(c.heads);
         p.tm[0] = k64;
         p.tm[1] = v64;
@@ -717,7 +714,7 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         p.tmA[1] = g128;
         p.out0 = c.dq;
         p.out0_stride = c.q_stride;
-        rc = c.hd <= 64 ? run<64, false>(p, num_sms, s, true) : run<128, false>(p, num_sms, s, true);
+        rc = c.hd <= 64 ? run<64, false>(p, units, num_sms, s, true) : run<128, false>(p, units, num_sms, s, true);
         if (rc) return rc;
     }
     if (keys) {
@@ -725,7 +722,7 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         p.partial = p.parts > 1 ? (float*)((char*)c.workspace + d_bytes(c)) : nullptr;
         const int64_t units = units_for(c, c.max_k, c.kv_heads * p.parts);
         if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
-        p.units = (int)units;
+        order_units(p, c, true, (c.max_k + kStand - 1) / kStand, c.chunk / kStand);
         p.by_fast = FastDiv::of(c.kv_heads * p.parts);
         p.by_parts = FastDiv::of(p.parts);
         p.tm[0] = q64;
@@ -736,12 +733,11 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         p.out0_stride = c.k_stride;
         p.out1 = c.dv;
         p.out1_stride = c.v_stride;
-        rc = c.hd <= 64 ? run<64, true>(p, num_sms, s, queries) : run<128, true>(p, num_sms, s, queries);
+        rc = c.hd <= 64 ? run<64, true>(p, units, num_sms, s, queries) : run<128, true>(p, units, num_sms, s, queries);
         if (rc) return rc;
         if (p.partial) {
-            const int64_t vecs = c.rows_k * c.kv_heads * c.hd / 4;
-            rc = (int)launch_k(k_attn_join, dim3((unsigned)((vecs + 255) / 256), 2), dim3(256), 0, s, true, (const float*)p.partial, p.parts, c.cu_k, c.n_seqs, c.rows_k, c.kv_heads,
-                               c.hd, c.dk, c.k_stride, c.dv, c.v_stride);
+            rc = (int)launch_k(k_attn_join, dim3((unsigned)((c.rows_k + kJoinRows - 1) / kJoinRows), 2), dim3(256), 0, s, true, (const float*)p.partial, p.parts, c.cu_k, c.n_seqs,
+                               c.rows_k, c.kv_heads, c.hd, c.dk, c.k_stride, c.dv, c.v_stride);
         }
     }
     return rc;
