@@ -100,10 +100,10 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
                 at.k = attn_span(p.cu_k[seq], p.cu_k[seq + 1], p.rows_k, p.max_k);
             }
             at.slots = slots_of(DKV ? at.k.len : at.q.len);
-            at.phase = 0;  // of the first query in its chunk
+            at.phase = 0;  // of the first query in its chunk, rounded down, so that the slots that see the end of one chunk and the start of the next come first
             if (!DKV && p.by_chunk_order) {
                 const int off = max(at.k.len - at.q.len, 0);
-                at.phase = min(slots_of(off - p.by_chunk.div(off) * p.chunk), p.period);
+                at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), p.period);
             }
             at.loaded = p.n_seqs <= 32;
         }

@@ -595,13 +595,13 @@ __global__ void __launch_bounds__(256) k_attn_dot(const bf16* __restrict__ d_out
     pdl_launch_dependents();
     const int64_t row0 = (int64_t)blockIdx.x * (4 * ROWS) + threadIdx.x / L;
     const int h = blockIdx.y, c = threadIdx.x % L * 8;
-    const int64_t begin = max(cu_q[0], 0), end = min((int64_t)cu_q[n_seqs], rows);
-    uint4 x[4], y[4];
+    const int64_t begin = cu_q[0], end = min((int64_t)cu_q[n_seqs], rows);
+    uint4 x[4], y[4];  // of rows in front of the first sequence and behind the last as well, which are not waited for to be told apart
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = row0 + i * ROWS;
         x[i] = y[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (row >= begin && row < end && c < hd) {
+        if (row < rows && c < hd) {
             x[i] = __ldg((const uint4*)(d_out + row * stride + (int64_t)h * hd + c));
             y[i] = __ldg((const uint4*)(out + row * stride + (int64_t)h * hd + c));
         }
@@ -629,8 +629,8 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* __restrict__ par
     const int per_row = kv_heads * hd / 4;
     const int64_t plane = rows * kv_heads * hd;
     const float* src = partial + (int64_t)blockIdx.y * parts * plane;
-    pdl_wait();
     const int begin = cu_k[0], end = cu_k[n_seqs];
+    pdl_wait();
     for (int i = threadIdx.x; i < kJoinRows * per_row; i += 256) {
         const int r = i / per_row, c = (i - r * per_row) * 4;
         const int64_t row = (int64_t)blockIdx.x * kJoinRows + r;
