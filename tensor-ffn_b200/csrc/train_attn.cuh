@@ -66,6 +66,12 @@ __device__ __forceinline__ void attn_visible(const AttnDev& p, int q_len, int k_
     }
 }
 
+// bits [lo, hi) of 64, whatever lo and hi
+__device__ __forceinline__ uint64_t bits_between(int lo, int hi) {
+    const int from = min(max(lo, 0), 64), to = min(max(hi, 0), 64);
+    return (to == 64 ? ~0ull : (1ull << to) - 1) & ~(from == 64 ? ~0ull : (1ull << from) - 1);
+}
+
 // Which units a block computes. A unit is (fast, sequence, slot): `slots_of` says how many slots a sequence has, and heads are fastest, so that blocks
 // that stream the same rows run together. The units that there are, empty ones not counted, stand in one order, longest first: by `level`, which is how
 // much of the other side a slot sees (its distance from the sequence's first block, or in a chunk from the chunk's), and then by sequence.

@@ -401,28 +401,18 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 }
                 wait(&s_full[group], ph);
                 F2 pr[kTile / 2];
-                if (!whole) {
-#pragma unroll 1
-                    for (int c = 0; c < kTile; c += 16) {
-                        const int from = min(max(c_lo - c, 0), 16), to = min(max(c_hi - c, 0), 16);
-                        if (__all_sync(0xffffffffu, from == 0 && to == 16)) continue;
-                        const uint32_t seen = (1u << to) - 1u & ~((1u << from) - 1u);
-                        uint32_t s[16];
-                        tmem_ld16(buf + c, s);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!(seen & 1u << i)) s[i] = 0xff800000u;
-                        tmem_st16(buf + c, s);
-                    }
-                    tc_wait_st();
-                }
+                uint64_t seen = 0;
+                if (!whole) seen = bits_between(c_lo, c_hi);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t s[2][16], v[16];
                     tmem_ld16(buf + half * 32, s[0]);
                     tmem_ld16(buf + half * 32 + 16, s[1]);
                     tc_wait_ld();
+                    if (!whole)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (!((uint32_t)(seen >> (half * 32)) & 1u << i)) s[i >> 4][i & 15] = 0xff800000u;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         float4 l4 = make_float4(nl, nl, nl, nl);
