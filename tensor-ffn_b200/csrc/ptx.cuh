@@ -75,6 +75,16 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
     return false;
 }
 
+// mbar_wait in the fewest instructions: a block whose warps all do something else runs at the rate at which instructions come where they do not fit
+// the instruction cache, and a loop that the compiler unrolls at every wait is much of that.
+__device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, int* status, int code) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kSpinLimit; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    dev_fail(status, code);
+    return false;
+}
+
 // ---------------------------------------------------------------- bulk copies (local memory, no multicast)
 // 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {

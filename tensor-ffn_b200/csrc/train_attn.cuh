@@ -159,16 +159,6 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
     return false;
 }
 
-// mbar_wait in the fewest instructions: a block whose warps all do something else runs at the rate at which instructions come where they do not fit
-// the instruction cache, and a loop that the compiler unrolls at every wait is much of that.
-__device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, int* status, int code) {
-#pragma unroll 1
-    for (uint32_t i = 0; i < kSpinLimit; ++i)
-        if (mbar_try_wait(bar, parity)) return true;
-    dev_fail(status, code);
-    return false;
-}
-
 // What one warp has worked out of a unit reaches the others through a few slots of shared memory, each with a barrier for the warps that read it
 // and one for the warp that fills it. A slot is free again when every reader has copied it.
 constexpr int kUnitSlots = 4;

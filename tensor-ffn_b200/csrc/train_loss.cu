@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
         __syncthreads();
         bool ok = true;
         for (int i = 0; i < pieces && ok; ++i) {
-            ok = mbar_wait(&landed[i], 0, p.status, DEV_ERR_FULL_WAIT);
+            ok = wait_barrier(&landed[i], 0, p.status, DEV_ERR_FULL_WAIT);
             const int to = min((i + 1) * (kPiece / 16), packs);
             for (int v = i * (kPiece / 16) + tid; v < to; v += THREADS) {
                 float f[P::N];

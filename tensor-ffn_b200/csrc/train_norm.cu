@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(block_of<TPR>(), Bwd<V, LAYER, TPR, N, L>::kPe
             rstd_next = rstd_in[row + step];
             if (LAYER) mean_next = mean_in[row + step];
         }
-        if (RING) ok = ok && mbar_wait(&full[stage], phase, status, DEV_ERR_FULL_WAIT);
+        if (RING) ok = ok && wait_barrier(&full[stage], phase, status, DEV_ERR_FULL_WAIT);
         const T* const src_d = RING ? ring + (size_t)stage * 3 * pitch + lead : dy + row * width;
         const T* const src_x = RING ? src_d + pitch : x + row * width;
         const T* const src_s = RING ? src_d + 2 * pitch : skip + row * width;
