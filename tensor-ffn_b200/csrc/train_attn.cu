@@ -13,6 +13,7 @@
 // What bounds it: 64 columns a head: the exponentials (8 192 a tile at 16 a cycle), a quarter of which therefore run as polynomials on the FMA
 // pipe; 128: the products (640 cycles a tile).
 #include "train_attn.cuh"
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <type_traits>
@@ -479,6 +480,11 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
+// slots of a chunk, where a block of 128 queries has heads / parts of them; a chunk without an end is as good as none
+int chunk_slots(const AttnCall& c, int heads, int parts) {
+    return c.chunk == 0 ? 0 : (int)std::min<int64_t>(std::max<int64_t>((int64_t)c.chunk / kStand * heads / parts, 1), 1 << 28);
+}
+
 template <int HD>
 int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     using C = Cfg<HD>;
@@ -490,7 +496,7 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;
     const int64_t units = (blocks * G + p.parts - 1) / p.parts * c.n_seqs * c.kv_heads;
     if (units >= 1 << 30 || blocks * G >= 1 << 30) return (int)cudaErrorInvalidValue;
-    order_units(p, c, false, (blocks * G + p.parts - 1) / p.parts, (int64_t)c.chunk / kStand * G / p.parts);
+    p.chunk_slots = chunk_slots(c, G, p.parts);
     p.by_fast = FastDiv::of(c.kv_heads);
     p.by_parts = FastDiv::of(p.parts);
     const cudaError_t e = allow_shared<k_attn_fwd<HD>>(C::SMEM);
@@ -515,7 +521,7 @@ AttnDev attn_dev(const AttnCall& c) {
     p.group = c.heads / c.kv_heads;
     p.by_group = FastDiv::of(p.group);
     p.by_chunk = FastDiv::of(c.chunk > 0 ? c.chunk : 1);
-    p.by_fast = p.by_parts = p.by_turns = FastDiv::of(1);
+    p.by_fast = p.by_parts = FastDiv::of(1);
     p.hd = c.hd;
     p.causal = c.causal;
     p.chunk = c.chunk;
@@ -525,16 +531,6 @@ AttnDev attn_dev(const AttnCall& c) {
     p.lse = c.lse;
     p.status = c.status;
     return p;
-}
-
-// slots: of the longest sequence; chunk_slots: of a chunk. Queries may begin in the middle of a chunk, so that they touch one more.
-void order_units(AttnDev& p, const AttnCall& c, bool keys, int64_t slots, int64_t chunk_slots) {
-    const int64_t period = c.chunk > 0 && chunk_slots < 1 ? 1 : chunk_slots;
-    p.by_chunk_order = c.chunk > 0 && period < slots;
-    p.period = (int)(p.by_chunk_order ? period : slots);
-    const int64_t turns = !p.by_chunk_order ? 1 : keys ? (slots + period - 1) / period : (slots + 2 * period - 1) / period;
-    p.by_turns = FastDiv::of(turns);
-    p.levels = (int)(turns * p.period);
 }
 
 bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box) {

@@ -31,8 +31,8 @@ struct AttnDev {
     const int *cu_q, *cu_k;
     int64_t rows_q, rows_k;
     int max_q, max_k, n_seqs, heads, kv_heads, group, hd, causal, chunk;  // group: query heads of a kv head
-    FastDiv by_fast, by_group, by_parts, by_chunk, by_turns;              // by_fast: units of a slot of a sequence
-    int levels, period, by_chunk_order;  // the order of the slots: levels = period * turns; by place in a chunk, or in the sequence
+    FastDiv by_fast, by_group, by_parts, by_chunk;                        // by_fast: units of a slot of a sequence
+    int chunk_slots;     // of a chunk, or 0
     int parts;           // units that a block takes at once (forward); parts of the query heads of a kv head (dK, dV)
     float scale, scale_log2;
     float* lse;          // [heads][rows_q]
@@ -82,9 +82,9 @@ struct AttnUnit {
     AttnSpan q, k;
 };
 struct AttnWalk {
+    int levels = -1, period, turns;                   // levels = period * turns: by place in a chunk and then by chunk, or by place in the sequence (one turn)
     int round = 0, level = 0, first = 0, before = 0;  // first: of 32 sequences; before: units in front of these of this level
-    bool loaded = false;                              // the lane's sequence is there and stays the same
-    int slots = 0, phase = 0;
+    int slots = 0, phase = 0;                         // of the lane's sequence
     AttnSpan q = {0, 0}, k = {0, 0};
 };
 // the block's next unit, for a whole warp: lane = sequence
@@ -92,34 +92,48 @@ template <bool DKV, typename F>
 __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUnit& u, F&& slots_of) {
     const int grid = gridDim.x, lane = threadIdx.x & 31;
     const int target = at.round * grid + (at.round & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
-    auto slot_of = [&](int level, int slots, int phase) {  // at most one of a sequence is at a level; -1 or more than there are: none
-        const int pos = p.by_turns.div(level), turn = level - pos * (int)p.by_turns.d;
-        return DKV && p.by_chunk_order ? turn * p.period + pos : slots - 1 - (turn * p.period + p.period - 1 - pos - phase);
-    };
-#pragma unroll 1
-    for (; at.level < p.levels;) {
-        if (!at.loaded) {
-            const int seq = at.first + lane;
-            at.q = at.k = {0, 0};
-            if (seq < p.n_seqs) {
-                at.q = attn_span(p.cu_q[seq], p.cu_q[seq + 1], p.rows_q, p.max_q);
-                at.k = attn_span(p.cu_k[seq], p.cu_k[seq + 1], p.rows_k, p.max_k);
-            }
-            at.slots = slots_of(DKV ? at.k.len : at.q.len);
-            at.phase = 0;  // of the first query in its chunk, rounded down, so that the slots that see the end of one chunk and the start of the next come first
-            if (!DKV && p.by_chunk_order) {
-                const int off = max(at.k.len - at.q.len, 0);
-                at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), p.period);
-            }
-            at.loaded = p.n_seqs <= 32;
+    auto load = [&](int seq) {
+        at.q = at.k = {0, 0};
+        if (seq < p.n_seqs) {
+            at.q = attn_span(p.cu_q[seq], p.cu_q[seq + 1], p.rows_q, p.max_q);
+            at.k = attn_span(p.cu_k[seq], p.cu_k[seq + 1], p.rows_k, p.max_k);
         }
-        if (at.loaded && p.n_seqs * p.n_seqs * (int64_t)p.by_fast.d < 3 * grid) {  // few units a level: 32 levels at a time, lane = level
-            const int level = at.level + lane;
+        at.slots = slots_of(DKV ? at.k.len : at.q.len);
+    };
+    if (at.levels < 0) {  // how long the longest sequence is: the call's bounds may be far above it
+        int most = 0;
+#pragma unroll 1
+        for (int first = 0; first < p.n_seqs; first += 32) {
+            load(first + lane);
+            most = max(most, at.slots);
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        const bool by_chunk = p.chunk_slots > 0 && p.chunk_slots < most;
+        at.period = by_chunk ? p.chunk_slots : most;
+        // queries may begin in the middle of a chunk, so that they touch one more
+        at.turns = !by_chunk ? 1 : (most + at.period - 1) / at.period + (DKV ? 0 : 1);
+        at.levels = at.period * at.turns;
+    }
+    const bool by_chunk = at.turns > 1, few = p.n_seqs <= 32;
+#pragma unroll 1
+    for (; at.level < at.levels;) {
+        if (!few) load(at.first + lane);
+        at.phase = 0;  // of the first query in its chunk, rounded down, so that the slots that see the end of one chunk and the start of the next come first
+        if (!DKV && by_chunk) {
+            const int off = max(at.k.len - at.q.len, 0);
+            at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), at.period);
+        }
+        // at most one slot of a sequence is at a level: this, unless it is negative or more than there are
+        auto slot_at = [&](int pos, int turn, int slots, int phase) {
+            return DKV && by_chunk ? turn * at.period + pos : slots - 1 - (turn * at.period + at.period - 1 - pos - phase);
+        };
+        if (few && p.n_seqs * p.n_seqs * (int64_t)p.by_fast.d < 3 * grid) {  // few units a level: 32 levels at a time, lane = level
+            const int level = at.level + lane, pos = by_chunk ? level / at.turns : level, turn = level - pos * at.turns;
             int sum = 0;
 #pragma unroll 1
             for (int i = 0; i < p.n_seqs; ++i) {
-                const int slots = __shfl_sync(0xffffffffu, at.slots, i), slot = slot_of(level, slots, __shfl_sync(0xffffffffu, at.phase, i));
-                sum += slot >= 0 && slot < slots && level < p.levels;
+                const int slots = __shfl_sync(0xffffffffu, at.slots, i), slot = slot_at(pos, turn, slots, __shfl_sync(0xffffffffu, at.phase, i));
+                sum += slot >= 0 && slot < slots && level < at.levels;
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -134,7 +148,7 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
             }
             if (!reach) continue;
         }
-        const int slot = slot_of(at.level, at.slots, at.phase);
+        const int pos = by_chunk ? at.level / at.turns : at.level, slot = slot_at(pos, at.level - pos * at.turns, at.slots, at.phase);
         const bool there = slot >= 0 && slot < at.slots;
         const unsigned all = __ballot_sync(0xffffffffu, there);
         const int rest = target - at.before, rank = p.by_fast.div(rest);
@@ -255,7 +269,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // host side (train_attn.cu)
 AttnDev attn_dev(const AttnCall& c);
-void order_units(AttnDev& p, const AttnCall& c, bool keys, int64_t slots, int64_t chunk_slots);
 bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box);
 
 }  // namespace tffn

@@ -676,6 +676,7 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
     float* const d = (float*)c.workspace;
     AttnDev p = attn_dev(c);
     p.d = d;
+    p.chunk_slots = c.chunk > 0 ? std::max(c.chunk / kStand, 1) : 0;
     // without keys or without queries: any valid map stands in, none of its rows is read
     CUtensorMap q64, g64, k64, v64, q128, g128, k128, v128;
     const AttnCall& a = c;
@@ -696,7 +697,6 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         if (rc) return rc;
         const int64_t units = units_for(c, c.max_q, c.heads);
         if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
-        order_units(p, c, false, (c.max_q + kStand - 1) / kStand, c.chunk / kStand);
         p.by_fast = FastDiv::of(c.heads);
         p.tm[0] = k64;
         p.tm[1] = v64;
@@ -712,7 +712,6 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         p.partial = p.parts > 1 ? (float*)((char*)c.workspace + d_bytes(c)) : nullptr;
         const int64_t units = units_for(c, c.max_k, c.kv_heads * p.parts);
         if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
-        order_units(p, c, true, (c.max_k + kStand - 1) / kStand, c.chunk / kStand);
         p.by_fast = FastDiv::of(c.kv_heads * p.parts);
         p.by_parts = FastDiv::of(p.parts);
         p.tm[0] = q64;

@@ -50,9 +50,10 @@ def test_every_query_sees_every_key():
 
 def test_bounds_longer_than_any_sequence():
     """max_q and max_k are bounds, not lengths"""
-    lens = lengths(6, 300, 5)
-    for chunk in (0, 128):
-        both(attn.make(lens, lens, 4, 2, 64, chunk=chunk, seed=5, max_q=5000, max_k=7000))
+    for n in (6, 80):
+        lens = lengths(n, 300, 5)
+        for chunk in (0, 128, 1 << 30):
+            both(attn.make(lens, lens, 4, 2, 64, chunk=chunk, seed=5, max_q=5000, max_k=2 ** 31 - 1))
 
 
 @pytest.mark.parametrize("dtype", norm.TYPES)
