@@ -9,8 +9,8 @@
 // Bound by HBM: logits are read once and gradients written once. A row of a 151 936-word vocabulary is 608 KB, so a thread-block cluster
 // holds it in its shared memory between the sum and the gradient: each block one slice, fetched by bulk copies in pieces of 16 KB that
 // are summed as they land; the blocks exchange (maximum, sum, x[y]) through distributed shared memory. Slices of 76 KB leave three
-// blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 434 us,
-// 5.0 TB/s; two slices of 101 KB 460 us).
+// blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 422 us,
+// 5.2 TB/s; blocks of 512 threads 434 us, and two of them an SM with slices of 108 KB 460 us; clusters of 14 with slices of 44 KB 454 us).
 #include "launch.h"
 #include "ptx.cuh"
 #include "train.h"
@@ -431,8 +431,8 @@ int pick_policy(const LossCall& c, int num_sms, cudaStream_t s) {
     const int64_t bytes = (int64_t)c.vocab * sizeof(T);
     const int blocks = blocks_of(bytes, c.rows, num_sms, kSharedSlice);
     const bool wide = ((uintptr_t)c.logits | (uintptr_t)c.d_logits) % 16 == 0 && c.stride * sizeof(T) % 16 == 0, small = bytes / blocks <= 24 * 1024;
-    if (wide) return small ? run_policy<T, 128, true>(c, blocks, s) : run_policy<T, 512, true>(c, blocks, s);
-    return small ? run_policy<T, 128, false>(c, blocks, s) : run_policy<T, 512, false>(c, blocks, s);
+    if (wide) return small ? run_policy<T, 128, true>(c, blocks, s) : run_policy<T, 256, true>(c, blocks, s);
+    return small ? run_policy<T, 128, false>(c, blocks, s) : run_policy<T, 256, false>(c, blocks, s);
 }
 
 }  // namespace
