@@ -403,7 +403,7 @@ int run_bwd(const NormCall& c, int num_sms, cudaStream_t s) {
         if (e != cudaSuccess) return (int)e;
     }
     int parts = (int)std::min<int64_t>((c.rows + RPB - 1) / RPB, std::min(kMaxParts, num_sms * B::kPerSm));
-    if (L == kShifted && c.rows > (int64_t)parts * RPB) parts = std::max(parts / V * V, 1);
+    if (L == kShifted && c.rows > (int64_t)parts * RPB) parts = (int)std::max<int64_t>(parts / V * V, std::min<int64_t>(V, (c.rows + RPB - 1) / RPB));
     const bool fold = c.dweight || c.dbias;
     float* part_w = c.dweight ? c.workspace : nullptr;
     float* part_b = c.dbias ? c.workspace + (size_t)parts * c.width : nullptr;
