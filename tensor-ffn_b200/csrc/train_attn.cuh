@@ -84,7 +84,7 @@ struct AttnUnit {
 struct AttnWalk {
     int levels = -1, period, turns;                   // levels = period * turns: by place in a chunk and then by chunk, or by place in the sequence (one turn)
     int round = 0, level = 0, first = 0, before = 0;  // first: of 32 sequences; before: units in front of these of this level
-    int slots = 0, phase = 0;                         // of the lane's sequence
+    int loaded = -1, slots = 0, phase = 0;            // the lane's sequence, of those from `loaded` on
     AttnSpan q = {0, 0}, k = {0, 0};
 };
 // the block's next unit, for a whole warp: lane = sequence
@@ -92,19 +92,26 @@ template <bool DKV, typename F>
 __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUnit& u, F&& slots_of) {
     const int grid = gridDim.x, lane = threadIdx.x & 31;
     const int target = at.round * grid + (at.round & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
-    auto load = [&](int seq) {
+    auto load = [&](int first) {
+        const int seq = first + lane;
+        at.loaded = first;
         at.q = at.k = {0, 0};
         if (seq < p.n_seqs) {
             at.q = attn_span(p.cu_q[seq], p.cu_q[seq + 1], p.rows_q, p.max_q);
             at.k = attn_span(p.cu_k[seq], p.cu_k[seq + 1], p.rows_k, p.max_k);
         }
         at.slots = slots_of(DKV ? at.k.len : at.q.len);
+        at.phase = 0;  // of the first query in its chunk, rounded down, so that the slots that see the end of one chunk and the start of the next come first
+        if (!DKV && p.chunk_slots > 0) {
+            const int off = max(at.k.len - at.q.len, 0);
+            at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), p.chunk_slots);
+        }
     };
     if (at.levels < 0) {  // how long the longest sequence is: the call's bounds may be far above it
         int most = 0;
 #pragma unroll 1
         for (int first = 0; first < p.n_seqs; first += 32) {
-            load(first + lane);
+            load(first);
             most = max(most, at.slots);
         }
         most = __reduce_max_sync(0xffffffffu, most);
@@ -114,20 +121,15 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
         at.turns = !by_chunk ? 1 : (most + at.period - 1) / at.period + (DKV ? 0 : 1);
         at.levels = at.period * at.turns;
     }
-    const bool by_chunk = at.turns > 1, few = p.n_seqs <= 32;
+    const bool by_chunk = at.turns > 1;
 #pragma unroll 1
     for (; at.level < at.levels;) {
-        if (!few) load(at.first + lane);
-        at.phase = 0;  // of the first query in its chunk, rounded down, so that the slots that see the end of one chunk and the start of the next come first
-        if (!DKV && by_chunk) {
-            const int off = max(at.k.len - at.q.len, 0);
-            at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), at.period);
-        }
+        if (at.loaded != at.first) load(at.first);
         // at most one slot of a sequence is at a level: this, unless it is negative or more than there are
         auto slot_at = [&](int pos, int turn, int slots, int phase) {
-            return DKV && by_chunk ? turn * at.period + pos : slots - 1 - (turn * at.period + at.period - 1 - pos - phase);
+            return DKV && by_chunk ? turn * at.period + pos : slots - 1 - (turn * at.period + at.period - 1 - pos - (by_chunk ? phase : 0));
         };
-        if (few && p.n_seqs * p.n_seqs * (int64_t)p.by_fast.d < 3 * grid) {  // few units a level: 32 levels at a time, lane = level
+        if (p.n_seqs <= 32 && p.n_seqs * p.n_seqs * (int64_t)p.by_fast.d < 3 * grid) {  // few units a level: 32 levels at a time, lane = level
             const int level = at.level + lane, pos = by_chunk ? level / at.turns : level, turn = level - pos * at.turns;
             int sum = 0;
 #pragma unroll 1

@@ -18,12 +18,18 @@
 //
 // A persistent block of three (64 columns a head) or two (128) groups of four warps, thread = standing row, so that a row's mask is an interval of
 // columns; the groups take turns at the tiles, one's exponentials under the others' products. Four more warps turn the accumulators into results
-// while the groups are at the next unit. One warp works out the units and fills the rings by TMA; one per group issues its products. The sums of all tiles go to the same accumulators: the product warps take turns at
-// them, each waiting for the one before, so that a row is always added up in one order.
+// while the groups are at the next unit. One warp works out the units and fills the rings by TMA; one per group issues its products.
+// The sums of all tiles go to the same accumulators: the product warps take turns at them, each waiting for the one before, so that a row
+// is always added up in one order.
 //
 // All these programs run at once, and short sequences go through all of their code all the time: what does not fit the instruction cache
-// is what such a call waits for (32 sequences of up to 512 queries, 14 / 2 heads of 64 columns: 112 us; with a mask variant of P and
-// unrolled waits 157 us; then with the results in the groups' hands 152 us).
+// is what such a call waits for (32 ragged sequences of up to 512 queries, 14 / 2 heads of 64 columns: 112 us; with a variant of P for masks and
+// unrolled waits 157 us, and then with the results in the groups' hands 152 us).
+//
+// What bounds it: 128 columns: the products, 1 280 cycles a tile (1 x 8 192, 28 / 4 heads: 1 350 us, 0.89 PFLOP/s counted as the five products that
+// there have to be, 1.4 as the eight that are formed, under the power limit); 64 columns: 640 cycles of products, 512 of exponentials and
+// as many of fp32 arithmetic in about 900 (8 x 4 096, 14 / 2 heads: 856 us, 0.70); short sequences: the chain S, P, dP, dS, product of a unit of few
+// tiles, and the calls around (the 32 sequences above, with the order of units of now: 77 us, of which dot products and joins 15).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cstring>

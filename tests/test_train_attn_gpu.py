@@ -3,8 +3,8 @@
 Tolerances are computed per element from the roundings that the kernels make, each at most half a step (2^-8 of a bf16 value):
   O    P enters its product as bf16: 2^-8 sum P |V|; O itself 2^-8 |O|
   dV   2^-8 sum P |dO|, and 2^-8 |dV|
-  dS   = P (dP - D): rounded to bf16, 2^-8 |dS|; D = dO . O with O as the forward call stored it: its error is at most
-       sum |dO| (2^-8 sum P |V| + 2^-8 |O|) and enters as P times that
+  dS   = P (dP - D): rounded to bf16, 2^-8 |dS|, about the D of the stored O, which is off by at most
+       sum |dO| (2^-8 sum P |V| + 2^-8 |O|): what it leaves out of dS enters as P times that
   dQ, dK  sums of (dS's errors) |K| or |Q| times the scale, and 2^-8 of the result
 What is fp32 (S, exponentials, sums) adds FP = 2^-10 of the same magnitudes: |S| < 64 here, so that rounding it costs an exponential at most
 64 * 2^-18 (64 products and a sum of 64 terms, each a rounding of 2^-24: 2^6 * 2^-24 of the sum of magnitudes, below 64 times 4)."""
