@@ -9,7 +9,7 @@
 // 8 192 x 2 048 bf16 take 14.3 us (4.7 TB/s; a row a warp 16.3 us). Backward: a persistent block walks over rows with the weight
 // and its own columns of dweight / dbias in registers, the next rows on their way into shared memory; its sums go to the workspace once
 // and a second kernel adds the blocks' sums per column in block order, so that the result does not depend on timing. 16 384 x 3 584 bf16
-// with skip take 77 us (6.1 TB/s; loads straight into registers 97 us), 4 099 x 1 111 fp32 of the layer norm 22 us (by single
+// with skip take 75 us (6.3 TB/s; loads straight into registers 97 us), 4 099 x 1 111 fp32 of the layer norm 22 us (by single
 // elements 29 us).
 #include "launch.h"
 #include "ptx.cuh"
@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(block_of<TPR>(), Bwd<V, LAYER, TPR, N, L>::kPe
 
 // column sums of the blocks' parts, in block order: kRuns runs of blocks per column, added in order
 constexpr int kRuns = 32;
+static_assert(kMaxParts % kRuns == 0, "");
 __global__ void __launch_bounds__(32 * kRuns) k_norm_fold(const float* part_w, const float* part_b, int parts, int width, float* dweight, float* dbias) {
     __shared__ float s[kRuns][33];
     pdl_wait();
@@ -366,9 +367,13 @@ __global__ void __launch_bounds__(32 * kRuns) k_norm_fold(const float* part_w, c
     float* out = blockIdx.y ? dbias : dweight;
     const int col = blockIdx.x * 32 + threadIdx.x, run = (parts + kRuns - 1) / kRuns, p0 = threadIdx.y * run, p1 = min(p0 + run, parts);
     float a = 0.f;
-    if (col < width)
-#pragma unroll 8
-        for (int p = p0; p < p1; ++p) a += part[(size_t)p * width + col];
+    if (col < width) {
+        float v[kMaxParts / kRuns];  // all of them in flight
+#pragma unroll
+        for (int i = 0; i < kMaxParts / kRuns; ++i) v[i] = p0 + i < p1 ? part[(size_t)(p0 + i) * width + col] : 0.f;
+#pragma unroll
+        for (int i = 0; i < kMaxParts / kRuns; ++i) a += v[i];
+    }
     s[threadIdx.y][threadIdx.x] = a;
     __syncthreads();
     if (threadIdx.y == 0 && col < width) {
