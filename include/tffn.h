@@ -258,8 +258,8 @@ int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const vo
  * q, k and v may be parts of one projection's output. Query heads share kv heads in groups of heads / kv_heads. The queries of a
  * sequence are its last positions: query j has position len_k - len_q + j, and with `causal` it sees the keys up to its own position
  * (none, if that is negative), with chunk > 0 (causal only) no key before position / chunk * chunk. A query that sees no key has
- * out = 0, lse = -inf and no gradient. Values inside a sequence have to be finite. max_q and max_k bound the lengths (rows beyond are not
- * computed); scale > 0. */
+ * out = 0, lse = -inf and no gradient. Values inside a sequence have to be finite. max_q and max_k bound the lengths (a longer sequence is
+ * cut to them: that is memory-safe, not a result); scale > 0. */
 typedef struct tffn_attention {
     int32_t n_seqs, heads, kv_heads, head_dim, max_q, max_k, causal, chunk;
     int64_t rows_q, rows_k; /* rows of the buffers */

@@ -29,7 +29,7 @@
 // What bounds it: 128 columns: the products, 1 280 cycles a tile (1 x 8 192, 28 / 4 heads: 1 350 us, 0.89 PFLOP/s counted as the five products that
 // there have to be, 1.4 as the eight that are formed, under the power limit); 64 columns: 640 cycles of products, 512 of exponentials and
 // as many of fp32 arithmetic in about 900 (8 x 4 096, 14 / 2 heads: 856 us, 0.70); short sequences: the chain S, P, dP, dS, product of a unit of few
-// tiles, and the calls around (the 32 sequences above, with the order of units of now: 77 us, of which dot products and joins 15).
+// tiles, and the calls around (the 32 sequences above, with the order of units of now and all heads of a kv head in one block: 73 us, of which dot products 10).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cstring>
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 accumulate(tmem + C::ACC, buf, DKV ? 1 : 0, at, !first);
                 umma_commit_elect(&p_added[g]);
                 have = find(1);
-                // 64 columns: six stages, the tile is as good as there; 128: four, dS comes first where it is not
+                // where the next tile is not there yet, dS comes first
                 early = have && (seen == item || there(&a_full[item % C::UNITS], (uint32_t)(item / C::UNITS) & 1u)) && there(&full[st], parity);
                 if (early) scores(0);
                 if (follows)
@@ -656,14 +656,16 @@ int run(const AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) 
 int64_t units_for(const AttnCall& c, int most, int fast) { return (int64_t)((most + kStand - 1) / kStand) * c.n_seqs * fast; }
 
 // Parts of the query heads of a kv head for dK, dV. One block adds all of them up where there are one and a half units of work for each of the
-// 148 SMs, as the packed rows let expect; else the heads are dealt to as many units as that takes, and their sums are joined through the workspace.
+// 148 SMs, as the packed rows let expect (one, if sequences are so short that the join costs as much as the last units); else the heads are dealt to as many units as that takes, and their sums are joined through the workspace.
 // All heads together against this, us, whole call: 1 x 4 096, 14 / 2 heads of 64 296 against 134; 8 ragged x 2 048, 12 / 2 of 128 228 against 175.
-// Parts of single heads against this: 8 x 4 096, 14 / 2 of 64 986 against 852; 1 x 8 192, 28 / 4 of 128 1 415 against 1 363.
+// One unit an SM against one and a half: 1 x 4 096, 14 / 2 of 64 168 against 137; 20 ragged x 1 000 of them 114 against 111, 24 x 700 87 against 91,
+// 32 x 512 73 against 79. Parts of single heads against this: 8 x 4 096, 14 / 2 of 64 986 against 852; 1 x 8 192, 28 / 4 of 128 1 415 against 1 363.
 int parts_of(const AttnCall& c) {
     const int G = c.heads / c.kv_heads;
     const int64_t most = units_for(c, c.max_k, c.kv_heads), expected = (c.rows_k / kStand + c.n_seqs / 2) * c.kv_heads, units = std::max<int64_t>(std::min(most, expected), 1);
+    const int64_t enough = c.max_k > 768 ? 148 * 3 / 2 : 148;
     int parts = 1;
-    while (parts < G && units * parts < 148 * 3 / 2) ++parts;
+    while (parts < G && units * parts < enough) ++parts;
     const int per = (G + parts - 1) / parts;
     return (G + per - 1) / per;
 }
