@@ -105,3 +105,44 @@ def test_norm_leaves_what_is_around_odd_rows(dtype):
     norm.check_forward(s, "rms", dtype, y, mean, rstd)
     for f in flat:
         assert (f[:front] == 5).all() and (f[-9:] == 5).all()
+
+
+def test_two_threads():
+    """calls of two host threads on streams and workspaces of their own"""
+    import threading
+
+    import tffn
+    import torch
+    lens = [[300, 5, 129], [64, 700]]
+    states = [attn.make(x, x, 6, 2, 64, seed=i) for i, x in enumerate(lens)]
+    norms = [norm.make(400, 896, "bfloat16", "rms", seed=i) for i in range(2)]
+    out, errors = [None, None], []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                stream = torch.cuda.current_stream()
+                ws = torch.empty(tffn.attention_backward_workspace(states[i]["shape"]), dtype=torch.uint8, device="cuda")
+                for _ in range(20):
+                    attn.forward(states[i], stream.cuda_stream)
+                    attn.backward(states[i], stream.cuda_stream, ws)
+                    out[i] = norm.forward(norms[i], "rms", "bfloat16", stream=stream.cuda_stream)
+                stream.synchronize()
+        except Exception as e:  # noqa: BLE001 - told to the test
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        attn.check(states[i])
+        norm.check_forward(norms[i], "rms", "bfloat16", *out[i])
+
+
+@pytest.mark.parametrize("lens,heads,kv,dim", [([700] * 24, 14, 2, 64), ([1000, 400, 30], 14, 2, 64), ([90] * 9, 16, 2, 128), ([800, 769], 6, 3, 128)])
+def test_parts_of_the_heads(lens, heads, kv, dim):
+    """dK and dV of all heads of a kv head in one block, and of some of them in several, evenly dealt and not"""
+    both(attn.make(lens, lens, heads, kv, dim, seed=20))
