@@ -288,7 +288,8 @@ int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_s
  * and d_logits = the gradient of loss (0 through the clipped branch; on a tie through the other one), dtype, row_stride apart; it may be
  * logits itself. weight [rows] carries the mask and the normalisation (NULL: 1). A row of weight 0, or whose target is not in the vocabulary,
  * is not read: its gradient, loss, logprob and kl are 0. loss [1] (needs row_loss), row_loss, logprob, kl [rows] and d_logits may be NULL. Masked
- * vocabulary entries (-inf or the type's lowest value) weigh nothing. Rows of up to 1.7 MB (TFFN_ERR_UNSUPPORTED beyond). */
+ * vocabulary entries (-inf or the type's lowest value) weigh nothing beside any other; a row whose entries are all at the lowest value has equal ones,
+ * as the formula says. Rows of up to 1.7 MB (TFFN_ERR_UNSUPPORTED beyond). */
 int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, const float* old_logprob,
                      const float* ref_logprob, const float* advantage, const float* weight, int64_t rows, int vocab, float clip_low, float clip_high,
                      float kl_coef, float* loss, float* row_loss, float* logprob, float* kl, void* d_logits, void* stream);

@@ -3,8 +3,11 @@
 //   ratio = exp(lp - old),  gain = min(ratio * A, clip(ratio, 1 - low, 1 + high) * A),  kl = exp(ref - lp) - (ref - lp) - 1
 //   row_loss = weight * (kl_coef * kl - gain)
 //   d_logits[j] = slope * ([j = y] - p[j]),  slope = weight * (kl_coef * (1 - exp(ref - lp)) - (ratio * A where gain is not the clipped one))
-// Keeping y out of S keeps lp and 1 - p[y] exact to rounding however likely y is. Exponentials and sums are fp32 (base 2, relative to a
-// running maximum that is an exact fp32 number), a row's few scalars 64-bit, so that a ratio next to its clip is on the right side.
+// Keeping y out of S keeps lp and 1 - p[y] exact to rounding however likely y is. Exponentials and sums are fp32, a row's few scalars 64-bit, so
+// that a ratio next to its clip is on the right side. An exponential is 2^((x[j] - m) log2 e), m a running maximum that is one of the logits: the
+// difference is exact next to the maximum and overflows to nothing but -inf, so that finite logits of any size, a row that is masked as a whole by
+// the type's lowest value among them, have the weights that the formula gives them. One fused x[j] log2 e - m log2 e would overflow there, and be
+// off by the rounding of m log2 e.
 //
 // Bound by HBM: logits are read once and gradients written once. A row of a 151 936-word vocabulary is 608 KB, so a thread-block cluster
 // holds it in its shared memory between the sum and the gradient: each block one slice, fetched by bulk copies in pieces of 16 KB that
@@ -12,6 +15,7 @@
 // blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 425 us,
 // 5.2 TB/s; blocks of 512 threads 434 us, and two of them an SM with slices of 108 KB 460 us; clusters of 14 with slices of 44 KB 454 us).
 #include "launch.h"
+#include "pair.cuh"
 #include "ptx.cuh"
 #include "train.h"
 #include <algorithm>
@@ -47,12 +51,12 @@ __device__ __forceinline__ float exp2_exact(float x) {
     return x < -126.f ? 0.f : y * __int_as_float(__float_as_int(t) << 23);
 }
 
-// running (maximum, sum) of 2^(x * log2 e), the maximum in base 2
+// running maximum, and sum of exp(x - maximum)
 struct Lse {
-    float m = -1e30f, s = 0.f;
+    float m = -FLT_MAX, s = 0.f;
     __device__ __forceinline__ void join(float m2, float s2) {
         const float top = fmaxf(m, m2);
-        s = s * exp2_exact(m - top) + s2 * exp2_exact(m2 - top);
+        s = s * exp2_exact((m - top) * kLog2e) + s2 * exp2_exact((m2 - top) * kLog2e);
         m = top;
     }
 };
@@ -101,6 +105,23 @@ __device__ __forceinline__ float load_one(const bf16* p) { return __bfloat162flo
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_one(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// exp(f[i] - m), two differences and two products an instruction (log-probabilities of 1 024 x 151 936 bf16: 64 us, one at a time 70)
+template <int N>
+__device__ __forceinline__ void weights(float (&f)[N], float m) {
+    if constexpr (N % 2 == 0) {
+        const F2 m2 = f2(-m, -m), k2 = f2(kLog2e, kLog2e);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            split2(mul2(add2(f2(f[i], f[i + 1]), m2), k2), f[i], f[i + 1]);
+            f[i] = exp2_fast(f[i]);
+            f[i + 1] = exp2_fast(f[i + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = exp2_fast((f[i] - m) * kLog2e);
+    }
+}
+
 // N values at indices first ..; the one at index `skip` is left out
 template <int N>
 __device__ __forceinline__ void take(Lse& l, const float (&f)[N], int first, int skip) {
@@ -111,13 +132,13 @@ __device__ __forceinline__ void take(Lse& l, const float (&f)[N], int first, int
         if ((unsigned)(skip - first) < (unsigned)N && first + i == skip) t[i] = -INFINITY;
         top = fmaxf(top, t[i]);
     }
-    const float top2 = top * kLog2e;
-    if (top2 > l.m) {
-        l.s *= exp2_fast(l.m - top2);
-        l.m = top2;
+    if (top > l.m) {
+        l.s *= exp2_fast((l.m - top) * kLog2e);
+        l.m = top;
     }
+    weights(t, l.m);
 #pragma unroll
-    for (int i = 0; i < N; ++i) l.s += exp2_fast(fmaf(t[i], kLog2e, -l.m));
+    for (int i = 0; i < N; ++i) l.s += t[i];
 }
 
 // the block's result, in every thread of its first warp
@@ -176,9 +197,7 @@ __device__ __forceinline__ RowSum cluster_join(const float* mine, uint32_t block
     return r;
 }
 // log of S / exp(x[y]); -inf where nothing but the token weighs. In logarithms, since a masked token's logit may be the type's lowest value
-__device__ __forceinline__ double log_odds_against(const RowSum& r) {
-    return log((double)r.rest.s) + (double)r.rest.m / (double)kLog2e - (double)r.token;
-}
+__device__ __forceinline__ double log_odds_against(const RowSum& r) { return log((double)r.rest.s) + ((double)r.rest.m - (double)r.token); }
 // -log(1 + odds)
 __device__ __forceinline__ double token_logprob(double log_odds) { return log_odds > 700.0 ? -log_odds : -log1p(exp(log_odds)); }
 
@@ -337,9 +356,9 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
         const double clipped = fmin(fmax(ratio, 1.0 - (double)p.clip_low), 1.0 + (double)p.clip_high) * adv;
         const double kl = expm1(away) - away, free = ratio * adv;
         const double slope = (double)weight * ((double)p.kl_coef * -expm1(away) - (free <= clipped ? free : 0.0));
-        // p[j] = 2^(x[j] log2 e - top) * share, top the larger of the two exponents so that nothing overflows
-        const float token = r.token * kLog2e, top = fmaxf(r.rest.m, token);
-        const double share = 1.0 / ((double)r.rest.s * exp2((double)r.rest.m - (double)top) + exp2((double)r.token * (double)kLog2e - (double)top));
+        // p[j] = exp(x[j] - top) * share, top the row's maximum
+        const float top = fmaxf(r.rest.m, r.token);
+        const double share = 1.0 / ((double)r.rest.s * exp((double)r.rest.m - (double)top) + exp((double)r.token - (double)top));
         if (tid == 0) {
             coef[0] = top;
             coef[1] = (float)(-slope * share);
@@ -359,8 +378,9 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
             float f[P::N];
             P::unpack(((const uint4*)x_s)[v], f);
             const int first = begin + v * P::N;
+            weights(f, top);
 #pragma unroll
-            for (int i = 0; i < P::N; ++i) f[i] = c * exp2_fast(fmaf(f[i], kLog2e, -top));
+            for (int i = 0; i < P::N; ++i) f[i] *= c;
             if ((unsigned)(y - first) < (unsigned)P::N)
 #pragma unroll
                 for (int i = 0; i < P::N; ++i)
@@ -368,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
             __stcs((uint4*)(dst + begin) + v, P::pack(f));
         }
         for (int i = packs * P::N + tid; i < n; i += THREADS)
-            store_one(dst + begin + i, begin + i == y ? own : c * exp2_fast(fmaf(load_one(x_s + i), kLog2e, -top)));
+            store_one(dst + begin + i, begin + i == y ? own : c * exp2_fast((load_one(x_s + i) - top) * kLog2e));
     }
     if (blocks > 1) cluster_wait();  // every block has read this one's result
 }
