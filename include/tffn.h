@@ -284,12 +284,13 @@ int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_s
 /* The clipped policy loss with a KL term, and its gradient, in one pass over the logits. Per row, with lp the target's log-probability:
  *   ratio = exp(lp - old_logprob), gain = min(ratio * advantage, clip(ratio, 1 - clip_low, 1 + clip_high) * advantage)
  *   kl = exp(ref_logprob - lp) - (ref_logprob - lp) - 1        (0 with ref_logprob NULL)
- *   row_loss = weight * (kl_coef * kl - gain), loss = sum of row_loss
+ *   row_loss = weight * (kl_coef * kl - gain), loss = sum of row_loss; with kl_coef 0 kl is reported and counts nothing, infinite or not
  * and d_logits = the gradient of loss (0 through the clipped branch; on a tie through the other one), dtype, row_stride apart; it may be
  * logits itself. weight [rows] carries the mask and the normalisation (NULL: 1). A row of weight 0, or whose target is not in the vocabulary,
  * is not read: its gradient, loss, logprob and kl are 0. loss [1] (needs row_loss), row_loss, logprob, kl [rows] and d_logits may be NULL. Masked
  * vocabulary entries (-inf or the type's lowest value) weigh nothing beside any other; a row whose entries are all at the lowest value has equal ones,
- * as the formula says. Rows of up to 1.7 MB (TFFN_ERR_UNSUPPORTED beyond). */
+ * as the formula says. A token whose exp(ref_logprob - lp) leaves fp32's range (88 below its reference; a masked one) has kl = inf, and with a
+ * kl_coef above 0 a loss and a gradient that are not finite. Rows of up to 1.7 MB (TFFN_ERR_UNSUPPORTED beyond). */
 int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, const float* old_logprob,
                      const float* ref_logprob, const float* advantage, const float* weight, int64_t rows, int vocab, float clip_low, float clip_high,
                      float kl_coef, float* loss, float* row_loss, float* logprob, float* kl, void* d_logits, void* stream);

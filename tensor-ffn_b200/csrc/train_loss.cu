@@ -354,8 +354,10 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
         const double log_odds = log_odds_against(r), lp = token_logprob(log_odds);
         const double adv = p.advantage[row], ratio = exp(lp - (double)p.old_logprob[row]), away = p.ref_logprob ? (double)p.ref_logprob[row] - lp : 0.0;
         const double clipped = fmin(fmax(ratio, 1.0 - (double)p.clip_low), 1.0 + (double)p.clip_high) * adv;
-        const double kl = expm1(away) - away, free = ratio * adv;
-        const double slope = (double)weight * ((double)p.kl_coef * -expm1(away) - (free <= clipped ? free : 0.0));
+        const double kl = away == INFINITY ? away : expm1(away) - away, free = ratio * adv;
+        // a divergence of weight zero may be infinite (a masked token), and counts nothing all the same
+        const double kl_loss = p.kl_coef == 0.f ? 0.0 : (double)p.kl_coef * kl, kl_slope = p.kl_coef == 0.f ? 0.0 : (double)p.kl_coef * -expm1(away);
+        const double slope = (double)weight * (kl_slope - (free <= clipped ? free : 0.0));
         // p[j] = exp(x[j] - top) * share, top the row's maximum
         const float top = fmaxf(r.rest.m, r.token);
         const double share = 1.0 / ((double)r.rest.s * exp((double)r.rest.m - (double)top) + exp((double)r.token - (double)top));
@@ -366,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
         }
         if (rank == 0 && tid == 0) {
             if (p.logprob) p.logprob[row] = (float)lp;
-            if (p.row_loss) p.row_loss[row] = (float)((double)weight * ((double)p.kl_coef * kl - fmin(free, clipped)));
+            if (p.row_loss) p.row_loss[row] = (float)((double)weight * (kl_loss - fmin(free, clipped)));
             if (p.kl) p.kl[row] = (float)kl;
         }
     }

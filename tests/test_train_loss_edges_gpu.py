@@ -98,3 +98,27 @@ def test_masked_rows_over_their_own_logits_and_of_weight_zero():
         settle(s, [0, 5])
         kept = shifted(s)
         loss.check(s, loss.policy(s, grad=s["x"]), x=kept)
+
+
+@pytest.mark.parametrize("dtype", loss.TYPES)
+@pytest.mark.parametrize("vocab", [100, 60000])
+def test_a_divergence_that_is_only_watched(vocab, dtype):
+    """kl_coef 0: the same bits as without a reference, also where the token is masked, or so far below its reference that the divergence is infinite"""
+    import torch
+    s = loss.make(8, vocab, dtype, seed=4)
+    at = torch.arange(8, device="cuda"), s["y"].long()
+    for r, v in ((1, -math.inf), (3, torch.finfo(s["x"].dtype).min), (4, -1000.0)):
+        s["x"][r, s["y"][r]] = v
+    lp = torch.log_softmax(s["x"].double(), -1)[at]
+    s["ref"][[1, 3, 4]] = -2.0
+    s["old"][[1, 3, 4]] = -3.0
+    got = loss.policy(s, beta=0.0)
+    without = loss.policy(dict(s, ref=None), beta=0.0)
+    for n in ("loss", "row_loss", "lp", "grad"):
+        assert got[n].isfinite().all() or n == "lp", n
+        assert torch.equal(got[n], without[n]), n
+    assert got["lp"][1] == -math.inf and got["kl"][[1, 3, 4]].eq(math.inf).all()
+    keep = [0, 2, 5, 6, 7]
+    away = s["ref"].double() - lp
+    kl = torch.expm1(away) - away
+    assert ((got["kl"].double() - kl)[keep].abs() <= (loss.SUM * torch.expm1(away).abs() + loss.SUM ** 2 + 2 ** -24 * kl)[keep] + 1e-12).all()
