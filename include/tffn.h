@@ -259,7 +259,8 @@ int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const vo
  * sequence are its last positions: query j has position len_k - len_q + j, and with `causal` it sees the keys up to its own position
  * (none, if that is negative), with chunk > 0 (causal only) no key before position / chunk * chunk. A query that sees no key has
  * out = 0, lse = -inf and no gradient. Values inside a sequence have to be finite. max_q and max_k bound the lengths (a longer sequence is
- * cut to them: that is memory-safe, not a result); scale > 0. */
+ * cut to them: that is memory-safe, not a result), and may be loose: a call's work is what its rows hold. TFFN_ERR_UNSUPPORTED where that could be
+ * 2^30 blocks of 128 rows of a head. scale > 0. */
 typedef struct tffn_attention {
     int32_t n_seqs, heads, kv_heads, head_dim, max_q, max_k, causal, chunk;
     int64_t rows_q, rows_k; /* rows of the buffers */

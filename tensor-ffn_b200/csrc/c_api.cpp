@@ -504,6 +504,9 @@ AttnCall attn_call(const tffn_attention* a) {
     c.chunk = a->chunk;
     return c;
 }
+void need_fit(bool fits) {
+    if (!fits) throw Error(kErrUnsupported, "attention of 2^30 or more blocks of 128 rows of a head");
+}
 void need_rows(std::initializer_list<const void*> tensors, int64_t rows) {
     for (const void* t : tensors) need((t || rows == 0) && aligned(t, 16), "a tensor is NULL or not 16-byte aligned");
 }
@@ -579,6 +582,7 @@ int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* c
                            void* out, float* lse, void* stream) {
     return guard([&] {
         AttnCall c = attn_call(a);
+        need_fit(attention_forward_fits(c));
         need(cu_q && cu_k, "NULL offsets");
         need_rows({q, out}, c.rows_q);
         need_rows({k, v}, c.rows_k);
@@ -596,7 +600,11 @@ int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* c
 }
 int64_t tffn_attention_backward_workspace(const tffn_attention* a) {
     int64_t bytes = 0;
-    const int rc = guard([&] { bytes = attention_workspace_bytes(attn_call(a)); });
+    const int rc = guard([&] {
+        const AttnCall c = attn_call(a);
+        need_fit(attention_backward_fits(c));
+        bytes = attention_workspace_bytes(c);
+    });
     return rc < 0 ? rc : bytes;
 }
 int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k, const void* v,
@@ -604,6 +612,7 @@ int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* 
                             void* stream) {
     return guard([&] {
         AttnCall c = attn_call(a);
+        need_fit(attention_backward_fits(c));
         need(cu_q && cu_k, "NULL offsets");
         need_rows({q, out, d_out, dq}, c.rows_q);
         need_rows({k, v, dk, dv}, c.rows_k);

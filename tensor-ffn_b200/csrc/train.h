@@ -86,6 +86,9 @@ struct AttnCall {
     int* status;
 };
 int64_t attention_workspace_bytes(const AttnCall& c);
+// Whether a pass has fewer than 2^30 units of work, by what its packed rows can hold; the launchers count on it.
+bool attention_forward_fits(const AttnCall& c);
+bool attention_backward_fits(const AttnCall& c);
 [[nodiscard]] int launch_attention_train_forward(const AttnCall& c, int num_sms, cudaStream_t s);
 [[nodiscard]] int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t s);
 

@@ -495,8 +495,9 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     // 467 against 411; 8 x 4 096, 14 heads of 64 390 against 319; 32 ragged x 512 of them 41 against 34; 3 x 2 777 of them in chunks of 1 024 44
     // against 75; 1 x 1 000 of them 16 against 37.
     p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;
-    const int64_t units = (blocks * G + p.parts - 1) / p.parts * c.n_seqs * c.kv_heads;
-    if (units >= 1 << 30 || blocks * G >= 1 << 30) return (int)cudaErrorInvalidValue;
+    const int64_t n = std::min<int64_t>(c.n_seqs, c.rows_q);  // sequences with rows
+    const int64_t units = std::min((blocks * G + p.parts - 1) / p.parts * c.n_seqs, blocks_of_rows(c, c.max_q, c.rows_q) * G / p.parts + n) * c.kv_heads;
+    p.units = (int)std::min(units, kMostUnits - 1);
     p.chunk_slots = chunk_slots(c, G, p.parts);
     p.by_fast = FastDiv::of(c.kv_heads);
     p.by_parts = FastDiv::of(p.parts);
@@ -533,6 +534,11 @@ AttnDev attn_dev(const AttnCall& c) {
     p.status = c.status;
     return p;
 }
+
+int64_t blocks_of_rows(const AttnCall& c, int most, int64_t rows) {
+    return std::min((int64_t)((most + kStand - 1) / kStand) * c.n_seqs, rows / kStand + std::min<int64_t>(c.n_seqs, rows));
+}
+bool attention_forward_fits(const AttnCall& c) { return blocks_of_rows(c, c.max_q, c.rows_q) * c.heads < kMostUnits; }
 
 bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box) {
     return make_tmap_2d(nullptr, tm, x, (uint64_t)rows, (uint64_t)hd, (uint64_t)stride, (uint32_t)box, (uint32_t)heads, (uint32_t)hd);

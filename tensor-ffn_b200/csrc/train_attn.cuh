@@ -34,6 +34,7 @@ struct AttnDev {
     int max_q, max_k, n_seqs, heads, kv_heads, group, hd, causal, chunk;  // group: query heads of a kv head
     FastDiv by_fast, by_group, by_parts, by_chunk;                        // by_fast: units of a slot of a sequence
     int chunk_slots;     // of a chunk, or 0
+    int units;           // of the call, at most: below 2^30, so that sums over units stay in 32 bits whatever the offsets say
     int parts;           // units that a block takes at once (forward); parts of the query heads of a kv head (dK, dV)
     float scale, scale_log2;
     float* lse;          // [heads][rows_q]
@@ -93,6 +94,7 @@ template <bool DKV, typename F>
 __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUnit& u, F&& slots_of) {
     const int grid = gridDim.x, lane = threadIdx.x & 31;
     const int target = at.round * grid + (at.round & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
+    if (target >= p.units) return false;
     auto load = [&](int first) {
         const int seq = first + lane;
         at.loaded = first;
@@ -248,6 +250,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // host side (train_attn.cu)
+constexpr int64_t kMostUnits = 1 << 30;
+// blocks of kStand rows that sequences of at most `most` rows can have, out of `rows`: each one's last block may be the only one that is not full
+int64_t blocks_of_rows(const AttnCall& c, int most, int64_t rows);
 AttnDev attn_dev(const AttnCall& c);
 bool map_heads(CUtensorMap* tm, const bf16* x, int64_t rows, int64_t stride, int heads, int hd, int box);
 

@@ -653,8 +653,6 @@ int run(const AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) 
     return (int)launch_k(k_attn_bwd<HD, DKV>, dim3((unsigned)(units < num_sms ? units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
 }
 
-int64_t units_for(const AttnCall& c, int most, int fast) { return (int64_t)((most + kStand - 1) / kStand) * c.n_seqs * fast; }
-
 // Parts of the query heads of a kv head for dK, dV. One block adds all of them up where there are one and a half units of work for each of the
 // 148 SMs, as the packed rows let expect (one, if sequences are so short that the join costs as much as the last units); else the heads are dealt to as many units as that takes, and their sums are joined through the workspace.
 // All heads together against this, us, whole call: 1 x 4 096, 14 / 2 heads of 64 296 against 134; 8 ragged x 2 048, 12 / 2 of 128 228 against 175.
@@ -662,7 +660,7 @@ int64_t units_for(const AttnCall& c, int most, int fast) { return (int64_t)((mos
 // 32 x 512 73 against 79. Parts of single heads against this: 8 x 4 096, 14 / 2 of 64 986 against 852; 1 x 8 192, 28 / 4 of 128 1 415 against 1 363.
 int parts_of(const AttnCall& c) {
     const int G = c.heads / c.kv_heads;
-    const int64_t most = units_for(c, c.max_k, c.kv_heads), expected = (c.rows_k / kStand + c.n_seqs / 2) * c.kv_heads, units = std::max<int64_t>(std::min(most, expected), 1);
+    const int64_t most = std::min((int64_t)((c.max_k + kStand - 1) / kStand) * c.n_seqs, kMostUnits) * c.kv_heads, expected = (c.rows_k / kStand + c.n_seqs / 2) * c.kv_heads, units = std::max<int64_t>(std::min(most, expected), 1);
     const int64_t enough = c.max_k > 768 ? 148 * 3 / 2 : 148;
     int parts = 1;
     while (parts < G && units * parts < enough) ++parts;
@@ -676,6 +674,10 @@ int64_t d_bytes(const AttnCall& c) { return ((int64_t)c.heads * c.rows_q * 4 + 2
 int64_t attention_workspace_bytes(const AttnCall& c) {
     const int parts = parts_of(c);
     return d_bytes(c) + (parts > 1 ? 2 * parts * c.rows_k * c.kv_heads * c.hd * 4 : 0);
+}
+
+bool attention_backward_fits(const AttnCall& c) {
+    return blocks_of_rows(c, c.max_q, c.rows_q) * c.heads < kMostUnits && blocks_of_rows(c, c.max_k, c.rows_k) * c.kv_heads * parts_of(c) < kMostUnits;
 }
 
 int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t s) {
@@ -703,8 +705,8 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         rc = lanes == 8 ? (int)launch_k(k_attn_dot<8>, grid, dim3(256), 0, s, false, c.d_out, (const bf16*)c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d)
                         : (int)launch_k(k_attn_dot<16>, grid, dim3(256), 0, s, false, c.d_out, (const bf16*)c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d);
         if (rc) return rc;
-        const int64_t units = units_for(c, c.max_q, c.heads);
-        if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
+        const int64_t units = blocks_of_rows(c, c.max_q, c.rows_q) * c.heads;
+        p.units = (int)units;
         p.by_fast = FastDiv::of(c.heads);
         p.tm[0] = k64;
         p.tm[1] = v64;
@@ -718,8 +720,8 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
     if (keys) {
         p.parts = parts_of(c);
         p.partial = p.parts > 1 ? (float*)((char*)c.workspace + d_bytes(c)) : nullptr;
-        const int64_t units = units_for(c, c.max_k, c.kv_heads * p.parts);
-        if (units >= 1 << 30) return (int)cudaErrorInvalidValue;
+        const int64_t units = blocks_of_rows(c, c.max_k, c.rows_k) * c.kv_heads * p.parts;
+        p.units = (int)units;
         p.by_fast = FastDiv::of(c.kv_heads * p.parts);
         p.by_parts = FastDiv::of(p.parts);
         p.tm[0] = q64;
