@@ -516,6 +516,7 @@ LossCall loss_call(int dtype, const void* logits, int64_t row_stride, const int3
     need(rows == 0 || (logits && targets), "NULL logits or targets");
     need_elements(dtype, {logits});
     if (rows > (int64_t)1 << 27) throw Error(kErrUnsupported, "more than 2^27 rows of logits");
+    if (vocab > kLossMaxVocab) throw Error(kErrUnsupported, "rows of logits of 2^31 elements");
     LossCall c;
     memset(&c, 0, sizeof c);
     c.f32 = dtype == TFFN_DTYPE_F32;

@@ -50,6 +50,7 @@ int64_t norm_workspace_floats(int64_t rows, int width);
 [[nodiscard]] int launch_norm_backward(const NormCall& c, int num_sms, cudaStream_t s);
 
 // log-probability of one token per row of logits, and the clipped policy loss on it
+constexpr int kLossMaxVocab = INT32_MAX - 4096;  // an index a block's threads past the end of a row fits an int
 struct LossCall {
     bool f32;
     const void* logits;  // [rows][stride]

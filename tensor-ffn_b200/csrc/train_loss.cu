@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(1024) k_loss_sum(const float* row_loss, int64_
 }
 
 // elements of a block's slice: an equal share, in whole 16-byte packs
-int slice_of(int vocab, int blocks, int per_pack) { return ((vocab + blocks - 1) / blocks + per_pack - 1) / per_pack * per_pack; }
+int64_t slice_of(int64_t vocab, int blocks, int per_pack) { return ((vocab + blocks - 1) / blocks + per_pack - 1) / per_pack * per_pack; }
 
 // Blocks of a row. Three slices fit an SM where the row allows it; with fewer rows than SMs a row is cut further, to pieces of 8 KB, so that
 // more SMs fetch it.
@@ -428,7 +428,7 @@ int blocks_of(int64_t bytes, int64_t rows, int num_sms, int64_t hold) {
 template <typename T, int THREADS, bool WIDE>
 int run_logprobs(const LossCall& c, int blocks, cudaStream_t s) {
     return (int)launch_k_cluster(k_token_logprobs<T, THREADS, WIDE>, dim3((unsigned)(c.rows * blocks)), dim3(THREADS), dim3(blocks), 0, s, false, (const T*)c.logits, c.stride,
-                                 c.vocab, (uint32_t)blocks, slice_of(c.vocab, blocks, Pack<T>::N), c.targets, c.logprob);
+                                 c.vocab, (uint32_t)blocks, (int)slice_of(c.vocab, blocks, Pack<T>::N), c.targets, c.logprob);
 }
 template <typename T>
 int pick_logprobs(const LossCall& c, int num_sms, cudaStream_t s) {
@@ -448,7 +448,7 @@ int run_policy(const LossCall& c, int blocks, cudaStream_t s) {
     p.rows = c.rows;
     p.stride = c.stride;
     p.vocab = c.vocab;
-    p.slice = slice_of(c.vocab, blocks, Pack<T>::N);
+    p.slice = (int)slice_of(c.vocab, blocks, Pack<T>::N);
     p.blocks = (uint32_t)blocks;
     p.targets = c.targets;
     p.old_logprob = c.old_logprob;
@@ -477,7 +477,7 @@ int pick_policy(const LossCall& c, int num_sms, cudaStream_t s) {
 
 }  // namespace
 
-bool policy_loss_supported(bool f32, int vocab) { return (int64_t)slice_of(vocab, kMaxBlocks, f32 ? 4 : 8) * (f32 ? 4 : 2) <= kMaxSlice; }
+bool policy_loss_supported(bool f32, int vocab) { return slice_of(vocab, kMaxBlocks, f32 ? 4 : 8) * (f32 ? 4 : 2) <= kMaxSlice; }
 
 int launch_token_logprobs(const LossCall& c, int num_sms, cudaStream_t s) {
     if (c.rows == 0) return 0;

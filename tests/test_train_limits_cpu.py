@@ -27,3 +27,13 @@ def test_units_that_cannot_be_counted():
     cpu.refused(-7, tffn.attention_backward_workspace, cpu.shape(**keys))
     cpu.no_device(cpu.attn, **keys)  # the forward call deals out blocks of queries only
     cpu.no_device(cpu.attn_back, size=1 << 50, **dict(many, n_seqs=1 << 20))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_vocabularies_next_to_2_31(dtype):
+    """sizes that a sum of a few more overflows: too long for the policy loss, and for log-probabilities where an index past the row does not fit"""
+    for vocab in (2 ** 31 - 1, 2 ** 31 - 6, 2 ** 31 - 4000):
+        cpu.refused(-7, cpu.policy, dtype=dtype, vocab=vocab)
+        cpu.refused(-7, cpu.logprob, dtype=dtype, vocab=vocab)
+    cpu.refused(-7, cpu.policy, dtype=dtype, vocab=2 ** 31 - 5000)
+    cpu.no_device(cpu.logprob, dtype=dtype, vocab=2 ** 31 - 5000)
