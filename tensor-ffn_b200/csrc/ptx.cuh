@@ -85,6 +85,13 @@ __device__ __forceinline__ bool wait_barrier(uint64_t* bar, uint32_t parity, int
     return false;
 }
 
+// After a wait that ran out, before the block ends: copies and products that are still on their way land in what is still this block's shared and
+// tensor memory. They take microseconds, this 10 ms.
+__device__ __forceinline__ void let_land() {
+#pragma unroll 1
+    for (int i = 0; i < 100; ++i) __nanosleep(100000);
+}
+
 // ---------------------------------------------------------------- bulk copies (local memory, no multicast)
 // 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_g2s(void* smem_dst, const void* gsrc, uint32_t bytes, uint64_t* bar) {

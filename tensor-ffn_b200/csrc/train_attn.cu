@@ -94,10 +94,10 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
     uint64_t* const k_full = (uint64_t*)(smem + C::BARS);
     uint64_t *const k_empty = k_full + MOST, *const v_full = k_empty + MOST, *const v_empty = v_full + MOST, *const q_full = v_empty + MOST, *const q_empty = q_full + NG,
                     *const s_full = q_empty + NG, *const s_free = s_full + NG, *const p_full = s_free + NG, *const o_full = p_full + NG, *const o_free = o_full + NG,
-                    *const u_full = o_free + NG, *const u_empty = u_full + kUnitSlots;
+                    *const joined = o_free + NG, *const u_full = joined + 2, *const u_empty = u_full + kUnitSlots;
     uint32_t* const tmem_slot = (uint32_t*)(u_empty + kUnitSlots);
     Units<NG>* const slots = (Units<NG>*)(smem + C::SLOTS);
-    static_assert((4 * MOST + 7 * NG + 2 * kUnitSlots) * 8 + 4 <= 640 && C::OWN_STAGES <= MOST, "");
+    static_assert((4 * MOST + 7 * NG + 2 + 2 * kUnitSlots) * 8 + 4 <= 640 && C::OWN_STAGES <= MOST, "");
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < MOST; ++i) {
@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
             mbar_init(&o_full[i], 1);
             mbar_init(&o_free[i], 128);
         }
+        for (int i = 0; i < 2; ++i) mbar_init(&joined[i], 4 * NG);
         for (int i = 0; i < kUnitSlots; ++i) {
             mbar_init(&u_full[i], 1);
             mbar_init(&u_empty[i], NG + 4 * NG);
@@ -157,10 +158,12 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
             }
         }
     };
+    bool ok = true;  // every wait of this warp so far has ended
     // a reader's copy of the index-th units of the block; false if there are no more
     auto take = [&](int index) {
         const int slot = index % kUnitSlots;
         const bool there = __all_sync(0xffffffffu, wait_barrier(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
+        ok = ok && there;
         w = slots[slot];
         __syncwarp();
         if (lane == 0) mbar_arrive(&u_empty[slot]);
@@ -171,7 +174,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         // ---- units, and by TMA their queries, then keys and values tile by tile
         const uint32_t base = smem_u32(smem);
         auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait_barrier(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
-        bool ok = true;
         int begun[NG] = {0};
         Place fill[NG];
         uint32_t first_round = (1u << NG) - 1u;  // of each part of the ring
@@ -228,7 +230,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         uint8_t* const ring = smem + ring_at + ring0 * C::STAGE;
         uint64_t *const kf = k_full + ring0, *const ke = k_empty + ring0, *const vf = v_full + ring0, *const ve = v_empty + ring0;
         const uint64_t q_d = umma_desc_k128(base + qb * C::Q_TILE), k_d = umma_desc_k128(smem_u32(ring)), v_d = umma_desc_n128(smem_u32(ring) + C::TILE, C::BLOCK);
-        bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, code)); };
         // two at once: a barrier that is ready costs 90 cycles to look at
         auto wait_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
@@ -312,12 +313,19 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + g * kTile, p_at = tmem + C::P + g * (kTile / 2), o_at = tmem + C::ACC + g * HD;
         uint8_t* const mine = smem + C::OUT + (warp - 4) * 2048;
         float2* const stats = (float2*)(smem + C::STATS);
-        bool ok = true;
-        // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers.
+        // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers. Those that the groups share are waits with
+        // a limit as well: a warp that never came to know of a unit has left, and does not reach them.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
         };
-        uint32_t turns = 0;  // tiles of this group so far
+        uint32_t turns = 0, shared = 0;  // tiles of this group so far; units that all groups have shared
+        auto join = [&](uint64_t* bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+            wait(bar, shared & 1u);
+            tc_fence_after();
+        };
         for (int index = 0; take(index); ++index) {
             if (own && g >= w.n) continue;
             int a_first = w.a_first[0], a_rows = w.a_rows[0], head = w.head[0];
@@ -425,9 +433,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                 weight[0] = sum > 0.f ? 1.f / sum : 0.f;
             } else {
                 stats[g * kStand + r] = make_float2(m, sum);
-                tc_fence_before();
-                named_barrier(1, NG * 128);
-                tc_fence_after();
+                join(&joined[0]);
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < NG; ++i) top = fmaxf(top, stats[i * kStand + r].x);
@@ -472,12 +478,15 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_fwd(const __grid_c
                 store_rows(mine, v, dst + c * 2, p.out0_stride * 2, a_rows - warp_row, (p.hd - c) / 8);
             }
             tc_fence_before();
-            if (!own) named_barrier(1, NG * 128);  // every group has read every O, and the statistics
+            if (!own) {  // every group has read every O, and the statistics
+                join(&joined[1]);
+                ++shared;
+            }
             if (any) mbar_arrive(&o_free[g]);
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(!ok)) let_land();
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 

@@ -243,7 +243,6 @@ __device__ __forceinline__ void store_rows(uint8_t* mine, const uint4 (&v)[4], c
     __syncwarp();
 }
 
-__device__ __forceinline__ void named_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *(const uint32_t*)&h;

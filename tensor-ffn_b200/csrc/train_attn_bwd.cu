@@ -94,7 +94,7 @@ struct Cfg {
     static constexpr int UNITS = HD == 64 ? 2 : 1;                        // units whose standing rows are there: what 227 KB hold next to the ring
     static constexpr int STAGES = HD == 64 ? 6 : 4;                       // at least two more than groups, for the loads on their way
     static constexpr int RING = UNITS * A_BYTES, OUT = RING + STAGES * STAGE; // OUT: 2 KB a warp for results on their way out
-    static constexpr int ROWS = OUT + 4 * 2048, ROWS_BYTES = GROUPS * 2 * kTile * 8;
+    static constexpr int ROWS = OUT + 4 * 2048, ROWS_BYTES = GROUPS * 4 * 2 * kTile * 8;
     static constexpr int SLOTS = ROWS + ROWS_BYTES, BARS = SLOTS + kUnitSlots * (int)sizeof(Unit), SMEM = BARS + 448;
     static constexpr int ACC = GROUPS * 2 * kTile;                        // tensor memory: S and dP of each group, then two accumulators
     static_assert(ACC + 2 * HD <= 512 && SMEM <= 227 * 1024 && STAGES > GROUPS && BARS % 8 == 0, "");
@@ -172,12 +172,14 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
     pdl_wait();
+    bool ok = true;  // every wait of this warp so far has ended
     // a reader's copy of the index-th unit of the block
     auto take = [&](int index) {
         const int slot = index % kUnitSlots;
         const bool there = __all_sync(0xffffffffu, wait_barrier(&u_full[slot], (uint32_t)(index / kUnitSlots) & 1u, p.status, DEV_ERR_FULL_WAIT));
         w = slots[slot];
         if (!there) w.tiles = -1;
+        ok = ok && there;
         __syncwarp();
         if (lane == 0) mbar_arrive(&u_empty[slot]);
         return w.tiles >= 0;
@@ -190,7 +192,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
             // ---- units, and by TMA their standing rows, then their tiles
             const uint32_t base = smem_u32(smem), bar = smem_u32(full), a_bar = smem_u32(a_full);
             auto wait = [&](uint64_t* b, uint32_t parity) { return __all_sync(0xffffffffu, wait_barrier(b, parity, p.status, DEV_ERR_EMPTY_WAIT)); };
-            bool ok = true;
             int item = 0, st = 0;
             uint32_t round = 0;
             for (int index = 0; ok; ++index) {
@@ -249,7 +250,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 static_assert(kTile == 64, "four products of 16 rows");
                 umma_bf16_ts_x4<8, 128>(d, a, n_d + (uint64_t)(uint32_t)((st * C::STAGE + which * C::TILE) >> 4), idesc_acc, more);
             };
-            bool ok = true;
             auto need = [&](uint64_t* bar, uint32_t parity, int code) { ok = ok && wait(bar, parity, code); };
             // Two of them, both at once where that is likely: a look at a barrier costs 90 cycles even if it is ready.
         auto need_both = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
@@ -351,8 +351,9 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         if (HD == 64) reg_inc<120>();
         const int group = (warp >> 2) - 1, r = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, buf = tmem + lanes + group * 2 * kTile;
-        float* const stats = (float*)(smem + C::ROWS) + group * 4 * kTile;  // -lse and -D of streamed queries, twice
-        bool ok = true;
+        // -lse and -D of streamed queries, twice. Each warp has its own: a barrier of the group's four would be one without a limit, or cost more than the loads
+        // (1 x 8 192, 28 / 4 heads of 128, whole backward pass: one copy behind a barrier in shared memory takes 4% longer).
+        float* const stats = (float*)(smem + C::ROWS) + (warp - 4) * 4 * kTile;
         // A wait that ran out lets the warp go on without waiting, since the others wait for it at their barriers.
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
@@ -381,18 +382,20 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                     ++h;
                 }
             };
-            // -lse (first half of the group) and -D (second half) of a tile's queries
+            // lse and D of a tile's queries, two each
+            float l_ahead[2] = {0.f, 0.f}, d_ahead[2] = {0.f, 0.f};
             auto fetch = [&]() {
-                const int col = w.first + in_head * kTile + (r & 63);
-                if (h >= w.h1 || col >= w.q_len) return 0.f;
+                const int col = w.first + in_head * kTile + lane;
                 const int64_t at = (int64_t)h * p.rows_q + w.q_first + col;
-                if (r >= 64) return -__ldcg(p.d + at);
-                const float l = __ldg(p.lse + at);
-                return l == -INFINITY ? 0.f : -l * kLog2e;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bool there = h < w.h1 && col + 32 * i < w.q_len;
+                    l_ahead[i] = there ? __ldg(p.lse + at + 32 * i) : -INFINITY;
+                    d_ahead[i] = there ? __ldcg(p.d + at + 32 * i) : 0.f;
+                }
             };
-            float ahead = 0.f;
             if (w.tiles > 0) settle();
-            if (DKV && t < w.tiles) ahead = fetch();
+            if (DKV && t < w.tiles) fetch();
             for (; t < w.tiles; t += NG, ++mine) {
                 const uint32_t ph = mine & 1u;
                 const int first = w.first + in_head * kTile, c_lo = lo - first, c_hi = hi - first;  // visible columns
@@ -401,9 +404,13 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
                 in_head += NG;
                 settle();
                 if (DKV) {
-                    q_stats[r] = ahead;
-                    ahead = fetch();
-                    named_barrier(1 + group, 128);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        q_stats[lane + 32 * i] = l_ahead[i] == -INFINITY ? 0.f : -l_ahead[i] * kLog2e;
+                        q_stats[kTile + lane + 32 * i] = -d_ahead[i];
+                    }
+                    fetch();
+                    __syncwarp();
                 }
                 wait(&s_full[group], ph);
                 F2 pr[kTile / 2];
@@ -489,7 +496,6 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         const int r = tid & 127, warp_row = (warp & 3) * 32;
         const uint32_t lanes = (uint32_t)warp_row << 16;
         uint8_t* const out = smem + C::OUT + (warp & 3) * 2048;
-        bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (ok) ok = __all_sync(0xffffffffu, wait_barrier(bar, parity, p.status, DEV_ERR_ACC_WAIT));
             tc_fence_after();
@@ -579,7 +585,7 @@ __global__ void __launch_bounds__(Cfg<HD>::THREADS, 1) k_attn_bwd(const __grid_c
         }
     }
     tc_fence_before();
-    __syncthreads();
+    if (__syncthreads_or(!ok)) let_land();
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 

@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(THREADS, THREADS > 128 ? kPerSm : 1) k_policy_
                 take(l, f, begin + v * P::N, y);
             }
         }
+        if (!ok) let_land();
     } else {
         for (int i = tid; i < n; i += THREADS) {
             x_s[i] = src[begin + i];

@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(block_of<TPR>(), Bwd<V, LAYER, TPR, N, L>::kPe
             phase ^= 1;
         }
     }
+    if (RING && !ok) let_land();
     if (!part_w && !part_b) return;
     // with kShifted rows each warp has columns of its own, so its sums are added by column in shared memory
     auto leave = [&](float(&a)[N][V], float* part) {
