@@ -295,7 +295,8 @@ int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_s
 int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, const float* old_logprob,
                      const float* ref_logprob, const float* advantage, const float* weight, int64_t rows, int vocab, float clip_low, float clip_high,
                      float kl_coef, float* loss, float* row_loss, float* logprob, float* kl, void* d_logits, void* stream);
-/* waits for the device and returns what the bounded waits of the training operators have reported on it so far (0: nothing) */
+/* Waits for the device, returns what the bounded waits of the training operators have reported on it since the last call (0: nothing; else the
+ * first of them) and clears it, so that a step can be told from the ones before. Callers that share a device share the word. */
 int tffn_train_status(int device);
 
 /* ---- kernel-level entry points used by the tests ---------------------------------------- */
@@ -328,7 +329,9 @@ int tffn_op_swiglu_bs1_noalloc(int device, void* h_io, const void* norm_w, const
 /* Runs a kernel that waits on a barrier nothing signals; returns the device status it
  * recorded (expected: 5). Proves that a wait that runs out returns instead of hanging. */
 int tffn_op_wait_selftest(int device);
-/* The same for the tensor-parallel hand-shake: one GPU plays rank 0 of a group of two whose peer never
+/* The same with the status word of the training operators: enqueued on the device's default stream, the code is what tffn_train_status returns next. */
+int tffn_op_train_wait_selftest(int device);
+/* The same as tffn_op_wait_selftest for the tensor-parallel hand-shake: one GPU plays rank 0 of a group of two whose peer never
  * signals; the kernel gives up after wait_ms (1..2000) and the recorded status is returned (expected: 7). */
 int tffn_op_tp_wait_selftest(int device, int wait_ms);
 

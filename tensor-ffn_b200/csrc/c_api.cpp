@@ -681,6 +681,10 @@ int tffn_train_status(int device) {
         int* word = status_word(device);
         TFFN_CUDA(cudaDeviceSynchronize());
         TFFN_CUDA(cudaMemcpy(&st, word, 4, cudaMemcpyDeviceToHost));
+        if (st != 0) {
+            TFFN_CUDA(cudaMemset(word, 0, 4));
+            TFFN_CUDA(cudaStreamSynchronize(nullptr));  // before the caller's next step can report
+        }
     });
     return rc < 0 ? rc : st;
 }
@@ -861,6 +865,14 @@ int tffn_op_wait_selftest(int device) {
         TFFN_CUDA(cudaMemcpy(&st, status.p, 4, cudaMemcpyDeviceToHost));
     });
     return rc < 0 ? rc : st;
+}
+
+int tffn_op_train_wait_selftest(int device) {
+    return guard([&] {
+        OnDevice on(device);
+        launch_wait_selftest(status_word(device), 0);
+        TFFN_CUDA(cudaGetLastError());
+    });
 }
 
 int tffn_op_tp_wait_selftest(int device, int wait_ms) {

@@ -1,5 +1,5 @@
 // The device status word of the training operators. Their kernels wait with a limit and run without the host waiting for them, so what
-// a wait that ran out has to say stays here until it is read (tffn_train_status).
+// a wait that ran out has to say stays here until it is read and cleared (tffn_train_status).
 #include "train.h"
 #include <mutex>
 

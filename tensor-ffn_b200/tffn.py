@@ -127,6 +127,7 @@ _SIGS = {
     "tffn_policy_loss": (_i, [_i, _i, _vp, _i64] + [_vp] * 5 + [_i64, _i, _f, _f, _f] + [_vp] * 6),
     "tffn_train_status": (_i, [_i]),
     "tffn_op_wait_selftest": (_i, [_i]),
+    "tffn_op_train_wait_selftest": (_i, [_i]),
     "tffn_op_tp_wait_selftest": (_i, [_i, _i]),
 }
 for _name, (_res, _args) in _SIGS.items():
@@ -554,7 +555,7 @@ def policy_loss(dtype: str, logits_ptr, targets_ptr, old_logprob_ptr, ref_logpro
 
 
 def train_status(device: int = 0) -> int:
-    """what the bounded waits of the training operators have reported (0: nothing); waits for the device"""
+    """what the bounded waits of the training operators have reported since the last call (0: nothing); waits for the device and clears it"""
     return _check(_L.tffn_train_status(device))
 
 
@@ -647,6 +648,10 @@ def op_swiglu_bs1_noalloc(h_io_ptr: int, norm_w_ptr: int, packed_base_ptr: int, 
 
 def op_wait_selftest(device: int = 0) -> int:
     return _check(_L.tffn_op_wait_selftest(device))
+
+
+def op_train_wait_selftest(device: int = 0):
+    _check(_L.tffn_op_train_wait_selftest(device))
 
 
 def op_tp_wait_selftest(wait_ms: int = 200, device: int = 0) -> int:
