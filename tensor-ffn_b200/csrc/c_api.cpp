@@ -474,6 +474,8 @@ NormCall norm_call(int kind, int dtype, const void* x, const void* weight, int64
 void need_elements(int dtype, std::initializer_list<const void*> tensors) {
     for (const void* t : tensors) need(aligned(t, dtype == TFFN_DTYPE_F32 ? 4 : 2), "a tensor is not aligned to its elements");
 }
+// fp32 or int32 tensors
+void need_words(std::initializer_list<const void*> tensors) { need_elements(TFFN_DTYPE_F32, tensors); }
 AttnCall attn_call(const tffn_attention* a) {
     need(a, "NULL attention");
     need(a->n_seqs >= 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->head_dim > 0, "bad attention heads or sequences");
@@ -515,6 +517,7 @@ LossCall loss_call(int dtype, const void* logits, int64_t row_stride, const int3
     need(rows >= 0 && vocab > 0 && (row_stride == 0 || row_stride >= vocab), "bad logits shape");
     need(rows == 0 || (logits && targets), "NULL logits or targets");
     need_elements(dtype, {logits});
+    need_words({targets});
     if (rows > (int64_t)1 << 27) throw Error(kErrUnsupported, "more than 2^27 rows of logits");
     if (vocab > kLossMaxVocab) throw Error(kErrUnsupported, "rows of logits of 2^31 elements");
     LossCall c;
@@ -538,6 +541,7 @@ int tffn_norm_forward(int device, int kind, int dtype, const void* x, const void
         need(y || rows == 0, "NULL output");
         need(c.layer ? bias != nullptr : !bias && !mean, "the layer norm needs a bias; the RMS norm has no bias and no mean");
         need_elements(dtype, {x, weight, bias, y});
+        need_words({mean, rstd});
         c.bias = bias;
         c.eps = eps;
         c.y = y;
@@ -563,6 +567,7 @@ int tffn_norm_backward(int device, int kind, int dtype, const void* dy, const vo
         need(rows == 0 || (dy && dx && rstd), "NULL gradient or rstd");
         need(c.layer ? mean || rows == 0 : !mean && !dbias, "the layer norm needs its mean; the RMS norm has no mean and no bias");
         need_elements(dtype, {dy, x, weight, skip, dx});
+        need_words({mean, rstd, dweight, dbias});
         if (dweight || dbias)
             need(rows == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= norm_workspace_floats(rows, width) * 4),
                  "norm workspace missing, not 16-byte aligned or too small");
@@ -585,6 +590,7 @@ int tffn_attention_forward(int device, const tffn_attention* a, const int32_t* c
         AttnCall c = attn_call(a);
         need_fit(attention_forward_fits(c));
         need(cu_q && cu_k, "NULL offsets");
+        need_words({cu_q, cu_k, lse});
         need_rows({q, out}, c.rows_q);
         need_rows({k, v}, c.rows_k);
         c.cu_q = cu_q;
@@ -615,6 +621,7 @@ int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* 
         AttnCall c = attn_call(a);
         need_fit(attention_backward_fits(c));
         need(cu_q && cu_k, "NULL offsets");
+        need_words({cu_q, cu_k, lse});
         need_rows({q, out, d_out, dq}, c.rows_q);
         need_rows({k, v, dk, dv}, c.rows_k);
         need(lse || c.rows_q == 0, "NULL lse");
@@ -642,6 +649,7 @@ int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_s
     return guard([&] {
         LossCall c = loss_call(dtype, logits, row_stride, targets, rows, vocab);
         need(logprob || rows == 0, "NULL output");
+        need_words({logprob});
         c.logprob = logprob;
         OnDevice on(device);
         check_launch(launch_token_logprobs(c, on.num_sms, (cudaStream_t)stream), "token log-probabilities");
@@ -656,6 +664,7 @@ int tffn_policy_loss(int device, int dtype, const void* logits, int64_t row_stri
         need(!loss || row_loss || rows == 0, "loss needs row_loss");
         need(clip_low >= 0.f && clip_low <= 1.f && clip_high >= 0.f && std::isfinite(clip_high) && std::isfinite(kl_coef), "bad clip range or KL coefficient");
         need_elements(dtype, {d_logits});
+        need_words({old_logprob, ref_logprob, advantage, weight, loss, row_loss, logprob, kl});
         if (!policy_loss_supported(c.f32, vocab)) throw Error(kErrUnsupported, "rows of logits of more than 1.7 MB");
         c.old_logprob = old_logprob;
         c.ref_logprob = ref_logprob;

@@ -37,3 +37,15 @@ def test_vocabularies_next_to_2_31(dtype):
         cpu.refused(-7, cpu.logprob, dtype=dtype, vocab=vocab)
     cpu.refused(-7, cpu.policy, dtype=dtype, vocab=2 ** 31 - 5000)
     cpu.no_device(cpu.logprob, dtype=dtype, vocab=2 ** 31 - 5000)
+
+
+@pytest.mark.parametrize("call,names", [
+    (cpu.norm, ("rstd",)), (lambda **kw: cpu.norm(kind="layer", bias=cpu.P, **kw), ("mean",)), (cpu.norm_back, ("rstd", "dweight")),
+    (lambda **kw: cpu.norm_back(**{**dict(kind="layer", mean=cpu.P, dbias=cpu.P), **kw}), ("mean", "dbias")), (cpu.attn, ("cu_q", "cu_k", "lse")),
+    (cpu.attn_back, ("cu_q", "cu_k", "lse")), (cpu.logprob, ("targets", "out")),
+    (cpu.policy, ("targets", "old", "ref", "advantage", "weight", "loss", "row_loss", "lp", "kl"))])
+def test_statistics_offsets_and_rows_start_on_their_elements(call, names):
+    """fp32 and int32 tensors half an element off: a fault on the device"""
+    for name in names:
+        assert "aligned" in cpu.refused(-1, call, **{name: cpu.ODD}), name
+    cpu.no_device(call, **{names[0]: cpu.P + 4})
