@@ -122,3 +122,16 @@ def test_a_divergence_that_is_only_watched(vocab, dtype):
     away = s["ref"].double() - lp
     kl = torch.expm1(away) - away
     assert ((got["kl"].double() - kl)[keep].abs() <= (loss.SUM * torch.expm1(away).abs() + loss.SUM ** 2 + 2 ** -24 * kl)[keep] + 1e-12).all()
+
+
+def test_no_advantage_and_a_ratio_out_of_range():
+    """an advantage of 0 gains nothing, also where the ratio is beyond all numbers"""
+    import torch
+    s = plain(200, "float32", 5, seed=5)
+    s["adv"] = torch.tensor([0.0, 0.0, 1.0, 0.0, -0.0], device="cuda")
+    s["old"][[0, 1, 2, 4]] = torch.tensor([-2000.0, -math.inf, -2000.0, -900.0], device="cuda")
+    got = loss.policy(s)
+    assert not got["row_loss"][[0, 1, 3, 4]].any() and not got["grad"].any()
+    want = -s["weight"][2].double() * (1 + 0.28)  # clipped
+    assert abs(got["row_loss"][2].double() - want) <= 2 ** -23 * abs(want)
+    assert abs(got["loss"][0].double() - want) <= 2 ** -23 * abs(want)
