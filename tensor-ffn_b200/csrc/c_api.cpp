@@ -483,7 +483,8 @@ AttnCall attn_call(const tffn_attention* a) {
     need(std::isfinite(a->scale) && a->scale > 0.f, "the attention scale must be positive");
     need(a->chunk >= 0 && (a->chunk == 0 || a->causal), "chunks need a causal mask");
     if (a->head_dim % 8 || a->head_dim > 128) throw Error(kErrUnsupported, "attention heads must be a multiple of 8 wide, at most 128");
-    if (a->heads > 65535 || a->rows_q > INT32_MAX - 4096 || a->rows_k > INT32_MAX - 4096) throw Error(kErrUnsupported, "more than 65535 heads or 2^31 rows");
+    if (a->heads > 65535 || a->rows_q > INT32_MAX - 4096 || a->rows_k > INT32_MAX - 4096 || a->n_seqs > INT32_MAX - 4096)
+        throw Error(kErrUnsupported, "more than 65535 heads or 2^31 rows or sequences");
     const int64_t q = (int64_t)a->heads * a->head_dim, k = (int64_t)a->kv_heads * a->head_dim;
     need(a->q_stride >= q && a->out_stride >= q && a->k_stride >= k && a->v_stride >= k, "an attention row stride is shorter than its row");
     need(a->q_stride % 8 == 0 && a->k_stride % 8 == 0 && a->v_stride % 8 == 0 && a->out_stride % 8 == 0, "attention row strides must be multiples of 8 elements");

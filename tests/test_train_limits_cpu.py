@@ -49,3 +49,12 @@ def test_statistics_offsets_and_rows_start_on_their_elements(call, names):
     for name in names:
         assert "aligned" in cpu.refused(-1, call, **{name: cpu.ODD}), name
     cpu.no_device(call, **{names[0]: cpu.P + 4})
+
+
+def test_sequences_next_to_2_31():
+    """the walk over the sequences steps 32 ahead: a count next to 2^31 would never be passed"""
+    for n in (2 ** 31 - 1, 2 ** 31 - 40):
+        cpu.refused(-7, cpu.attn, n_seqs=n)
+        cpu.refused(-7, cpu.attn_back, n_seqs=n)
+        cpu.refused(-7, tffn.attention_backward_workspace, cpu.shape(n_seqs=n))
+    cpu.no_device(cpu.attn, n_seqs=1 << 30)
