@@ -506,13 +506,13 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;
     const int64_t n = std::min<int64_t>(c.n_seqs, c.rows_q);  // sequences with rows
     const int64_t units = std::min((blocks * G + p.parts - 1) / p.parts * c.n_seqs, blocks_of_rows(c, c.max_q, c.rows_q) * G / p.parts + n) * c.kv_heads;
-    p.units = (int)std::min(units, kMostUnits - 1);
+    const unsigned grid = set_units(p, units, num_sms);
     p.chunk_slots = chunk_slots(c, G, p.parts);
     p.by_fast = FastDiv::of(c.kv_heads);
     p.by_parts = FastDiv::of(p.parts);
     const cudaError_t e = allow_shared<k_attn_fwd<HD>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_k(k_attn_fwd<HD>, dim3((unsigned)(units < num_sms ? units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, false, p);
+    return (int)launch_k(k_attn_fwd<HD>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, s, false, p);
 }
 
 }  // namespace
@@ -546,6 +546,12 @@ AttnDev attn_dev(const AttnCall& c) {
 
 int64_t blocks_of_rows(const AttnCall& c, int most, int64_t rows) {
     return std::min((int64_t)((most + kStand - 1) / kStand) * c.n_seqs, rows / kStand + std::min<int64_t>(c.n_seqs, rows));
+}
+unsigned set_units(AttnDev& p, int64_t units, int num_sms) {
+    p.units = (int)std::min(units, kMostUnits - 1);
+    const int grid = std::min(p.units, num_sms), groups = (p.n_seqs + 31) / 32;
+    p.most_levels = groups <= 1 ? INT32_MAX : std::max(32, 4 * (p.units / grid)) / groups;  // 32 sequences are one order either way
+    return (unsigned)grid;
 }
 bool attention_forward_fits(const AttnCall& c) { return blocks_of_rows(c, c.max_q, c.rows_q) * c.heads < kMostUnits; }
 

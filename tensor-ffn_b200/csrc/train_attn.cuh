@@ -34,6 +34,7 @@ struct AttnDev {
     int max_q, max_k, n_seqs, heads, kv_heads, group, hd, causal, chunk;  // group: query heads of a kv head
     FastDiv by_fast, by_group, by_parts, by_chunk;                        // by_fast: units of a slot of a sequence
     int chunk_slots;     // of a chunk, or 0
+    int most_levels;     // that the units of all sequences are looked at on: AttnWalk
     int units;           // of the call, at most: below 2^30, so that sums over units stay in 32 bits whatever the offsets say
     int parts;           // units that a block takes at once (forward); parts of the query heads of a kv head (dK, dV)
     float scale, scale_log2;
@@ -79,11 +80,16 @@ __device__ __forceinline__ uint64_t bits_between(int lo, int hi) {
 // much of the other side a slot sees (its distance from the sequence's first block, or in a chunk from the chunk's), and then by sequence.
 // A block has one of every round of `grid` units, in every other round counted from the end, so that the blocks end together.
 // 1 x 8 192, 28 heads of 128, forward: 411 us, with rounds counted from the start 469; 32 ragged x 512, 14 heads of 64, backward 80 us, else 112.
+//
+// A look at 32 sequences at one level costs 0.2 us, and all of them at every level is sequences x longest: one of 8 192 among 4 095 of 64 would be 1.3 ms of
+// looking (and a million of them long enough for the waits of the others to run out). Where that is more than four looks a unit, each 32 sequences are in
+// that order by themselves, one after the other, which is as many looks as there are units at most (those 4 096: forward 0.29 ms).
 struct AttnUnit {
     int fast, slot;
     AttnSpan q, k;
 };
 struct AttnWalk {
+    bool apart = false;                               // each 32 sequences by themselves
     int levels = -1, period, turns;                   // levels = period * turns: by place in a chunk and then by chunk, or by place in the sequence (one turn)
     int round = 0, level = 0, first = 0, before = 0;  // first: of 32 sequences; before: units in front of these of this level
     int loaded = -1, slots = 0, phase = 0;            // the lane's sequence, of those from `loaded` on
@@ -110,6 +116,14 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
             at.phase = min(slots_of((off - p.by_chunk.div(off) * p.chunk) / kStand * kStand), p.chunk_slots);
         }
     };
+    auto measure = [&](int most) {
+        most = __reduce_max_sync(0xffffffffu, most);
+        const bool by_chunk = p.chunk_slots > 0 && p.chunk_slots < most;
+        at.period = by_chunk ? p.chunk_slots : most;
+        // queries may begin in the middle of a chunk, so that they touch one more
+        at.turns = !by_chunk ? 1 : (most + at.period - 1) / at.period + (DKV ? 0 : 1);
+        at.levels = at.period * at.turns;
+    };
     if (at.levels < 0) {  // how long the longest sequence is: the call's bounds may be far above it
         int most = 0;
 #pragma unroll 1
@@ -117,16 +131,24 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
             load(first);
             most = max(most, at.slots);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
-        const bool by_chunk = p.chunk_slots > 0 && p.chunk_slots < most;
-        at.period = by_chunk ? p.chunk_slots : most;
-        // queries may begin in the middle of a chunk, so that they touch one more
-        at.turns = !by_chunk ? 1 : (most + at.period - 1) / at.period + (DKV ? 0 : 1);
-        at.levels = at.period * at.turns;
+        measure(most);
+        at.apart = at.levels > p.most_levels;
+        if (at.apart) {
+            load(0);
+            measure(at.slots);
+        }
     }
-    const bool by_chunk = at.turns > 1;
 #pragma unroll 1
-    for (; at.level < at.levels;) {
+    for (;;) {
+        if (at.level >= at.levels) {
+            at.first += 32;
+            if (!at.apart || at.first >= p.n_seqs) return false;
+            load(at.first);
+            measure(at.slots);
+            at.level = 0;
+            continue;
+        }
+        const bool by_chunk = at.turns > 1;
         if (at.loaded != at.first) load(at.first);
         // at most one slot of a sequence is at a level: this, unless it is negative or more than there are
         auto slot_at = [&](int pos, int turn, int slots, int phase) {
@@ -169,13 +191,16 @@ __device__ __forceinline__ bool next_unit(const AttnDev& p, AttnWalk& at, AttnUn
             return true;
         }
         at.before += __popc(all) * (int)p.by_fast.d;
+        if (at.apart) {
+            ++at.level;
+            continue;
+        }
         at.first += 32;
         if (at.first >= p.n_seqs) {
             at.first = 0;
             ++at.level;
         }
     }
-    return false;
 }
 
 // What one warp has worked out of a unit reaches the others through a few slots of shared memory, each with a barrier for the warps that read it
@@ -249,6 +274,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // host side (train_attn.cu)
+// units of a launch, its grid, and how many levels all sequences are looked at on
+unsigned set_units(AttnDev& p, int64_t units, int num_sms);
 constexpr int64_t kMostUnits = 1 << 30;
 // blocks of kStand rows that sequences of at most `most` rows can have, out of `rows`: each one's last block may be the only one that is not full
 int64_t blocks_of_rows(const AttnCall& c, int most, int64_t rows);

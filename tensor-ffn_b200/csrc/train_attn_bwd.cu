@@ -652,11 +652,11 @@ __global__ void __launch_bounds__(256) k_attn_join(const float* __restrict__ par
 }
 
 template <int HD, bool DKV>
-int run(const AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) {
+int run(AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) {
     using C = Cfg<HD>;
     const cudaError_t e = allow_shared<k_attn_bwd<HD, DKV>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3((unsigned)(units < num_sms ? units : num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
+    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3(set_units(p, units, num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
 }
 
 // Parts of the query heads of a kv head for dK, dV. One block adds all of them up where there are one and a half units of work for each of the
@@ -712,7 +712,6 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
                         : (int)launch_k(k_attn_dot<16>, grid, dim3(256), 0, s, false, c.d_out, (const bf16*)c.out, c.out_stride, c.cu_q, c.n_seqs, c.rows_q, c.heads, c.hd, d);
         if (rc) return rc;
         const int64_t units = blocks_of_rows(c, c.max_q, c.rows_q) * c.heads;
-        p.units = (int)units;
         p.by_fast = FastDiv::of(c.heads);
         p.tm[0] = k64;
         p.tm[1] = v64;
@@ -727,7 +726,6 @@ int launch_attention_train_backward(const AttnCall& c, int num_sms, cudaStream_t
         p.parts = parts_of(c);
         p.partial = p.parts > 1 ? (float*)((char*)c.workspace + d_bytes(c)) : nullptr;
         const int64_t units = blocks_of_rows(c, c.max_k, c.rows_k) * c.kv_heads * p.parts;
-        p.units = (int)units;
         p.by_fast = FastDiv::of(c.kv_heads * p.parts);
         p.by_parts = FastDiv::of(p.parts);
         p.tm[0] = q64;

@@ -43,3 +43,62 @@ def test_offsets_that_go_back_and_forth(dim):
         both(s)
         torch.cuda.synchronize()
         assert tffn.train_status() == 0
+
+
+MANY = [([5] * 200 + [1500] + [17] * 300, 0, 0), ([1] * 1500 + [130, 0, 900], 100, 256), ([0, 40] * 100 + [1100] + [64] * 37, 30, 200),
+        ([2] * 4000 + [700], 0, 128)]
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(14, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("lens,prefix,chunk", MANY)
+def test_many_short_sequences_and_a_long_one(lens, prefix, chunk, heads, kv, dim):
+    """each 32 sequences in an order of their own; twice the same bits"""
+    import torch
+    s = attn.make(lens, [n + (i * 7 % (prefix + 1)) for i, n in enumerate(lens)], heads, kv, dim, chunk=chunk, seed=len(lens))
+    first = both(s)
+    long = max(range(len(lens)), key=lambda i: lens[i])
+    near = [i for i in range(len(lens)) if lens[i] and (abs(i - long) < 20 or i < 20 or i % 97 == 0)]
+    check_some(s, near)
+    for name, t in both(s).items():
+        assert torch.equal(first[name], t), name
+
+
+def check_some(s, chosen):
+    """the oracle on some sequences, moved together"""
+    import torch
+    lens_q, lens_k = s["lens"]
+    at_q, at_k = [0], [0]
+    for a, b in zip(lens_q, lens_k):
+        at_q.append(at_q[-1] + a)
+        at_k.append(at_k[-1] + b)
+    rows_q = torch.cat([torch.arange(at_q[i], at_q[i + 1], device="cuda") for i in chosen])
+    rows_k = torch.cat([torch.arange(at_k[i], at_k[i + 1], device="cuda") for i in chosen])
+    part = {n: s[n][rows_q] for n in ("q", "dout", "out", "dq")} | {n: s[n][rows_k] for n in ("k", "v", "dk", "dv")}
+    attn.check(dict(part, lse=s["lse"][:, rows_q], lens=([lens_q[i] for i in chosen], [lens_k[i] for i in chosen]), shape=s["shape"]))
+    assert (s["out"][at_q[-1]:] == 5).all() and (s["dq"][at_q[-1]:] == 5).all() and (s["dk"][at_k[-1]:] == 5).all()
+    for n in ("out", "dq", "dk", "dv"):  # no row of any sequence is left as it was
+        rows = at_q[-1] if n in ("out", "dq") else at_k[-1]
+        assert not (s[n][:rows] == 5).flatten(1).all(1).any(), n
+
+
+def test_time_goes_by_the_rows():
+    """one long sequence among thousands of short ones takes about what the same rows take in a few: not sequences times longest (ten times as long)"""
+    import tffn
+    import torch
+
+    def time(lens):
+        s = attn.make(lens, lens, 2, 1, 64, seed=1)
+        ws = torch.empty(tffn.attention_backward_workspace(s["shape"]), dtype=torch.uint8, device="cuda")
+        stream, best = torch.cuda.current_stream().cuda_stream, 1e9
+        for _ in range(4):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            attn.forward(s, stream)
+            attn.backward(s, stream, ws)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        assert tffn.train_status() == 0
+        return best
+    few, many = time([2000] * 32 + [8192]), time([16] * 2000 + [8192] + [16] * 2000)
+    assert many < 3 * few, (few, many)
