@@ -279,7 +279,7 @@ int tffn_attention_backward(int device, const tffn_attention* a, const int32_t* 
                             int64_t workspace_bytes, void* stream);
 
 /* logprob[r] = log softmax(logits[r])[targets[r]], fp32; 0 where the target is not in 0 .. vocab - 1. logits: dtype [rows][vocab], rows
- * row_stride elements apart (0: vocab). What a policy sampled with, or a reference model says of the same tokens. */
+ * row_stride elements apart (0: vocab; vocab below 2^31 - 4096). What a policy sampled with, or a reference model says of the same tokens. */
 int tffn_token_logprobs(int device, int dtype, const void* logits, int64_t row_stride, const int32_t* targets, int64_t rows, int vocab, float* logprob,
                         void* stream);
 /* The clipped policy loss with a KL term, and its gradient, in one pass over the logits. Per row, with lp the target's log-probability:

@@ -7,12 +7,12 @@
 // heads of the same queries, which share what is fetched. S = Q K^T and O += P V are tcgen05 products. One warp works out the units and fills the
 // rings by TMA, one per group issues its products. S has its columns to itself and P others, so the next S is formed as soon as a group has S
 // in registers, and a group's exponentials follow each other without waiting for the tensor cores. The next unit's queries and scores are on their
-// way while results are stored. S, sums and O are fp32; P enters its product as bf16 (half a step, 2^-9 of each term, as inputs and results
+// way while results are stored. S, sums and O are fp32; P enters its product as bf16 (half a step, up to 2^-8 of each term, as inputs and results
 // have). A row's reference maximum moves only when it would be passed by more than 2^8, so O is rarely rescaled.
 //
 // What bounds it: 64 columns a head: the exponentials (8 192 a tile at 16 a cycle), a quarter of which therefore run as polynomials on the FMA
-// pipe (8 x 4 096, 14 / 2 heads: 316 us, 0.76 PFLOP/s); 128: the products (640 cycles a tile; 1 x 8 192, 28 / 4 heads: 411 us, 1.17 PFLOP/s); short
-// sequences: the chain from a unit's queries to its results (32 ragged x 512, 14 / 2 heads of 64: 31 us, 0.17).
+// pipe (8 x 4 096, 14 / 2 heads: 325 us, 0.74 PFLOP/s); 128: the products (640 cycles a tile; 1 x 8 192, 28 / 4 heads: 458 us, 1.05 PFLOP/s in a row of
+// calls, under the power limit); short sequences: the chain from a unit's queries to its results (32 ragged x 512, 14 / 2 heads of 64: 30 us, 0.17).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cmath>
@@ -500,7 +500,7 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     using C = Cfg<HD>;
     const int G = c.heads / c.kv_heads;
     const int64_t blocks = (c.max_q + kStand - 1) / kStand, all = blocks * c.n_seqs * c.heads;
-    // Units to themselves where every group of every SM gets four, us (one unit at a time against units of their own): 1 x 8 192, 28 heads of 128
+    // Units to themselves where every group of every SM gets four, counted by the bounds (ragged sequences have fewer: 32 x 512 2.6), us (one unit at a time against units of their own): 1 x 8 192, 28 heads of 128
     // 467 against 411; 8 x 4 096, 14 heads of 64 390 against 319; 32 ragged x 512 of them 41 against 34; 3 x 2 777 of them in chunks of 1 024 44
     // against 75; 1 x 1 000 of them 16 against 37.
     p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;

@@ -218,7 +218,8 @@ __device__ __forceinline__ void load_head(const CUtensorMap* tm, uint32_t dst, i
             tma_load_2d_elect(dst + i * block, tm, i * 64, row, bar);
 }
 // Zeros in rows [valid, rows) of `blocks` blocks of 128-byte rows, by a whole warp: rows behind a sequence weigh zero, but what lies there
-// may not be finite. For operands that only the calling warp's products read.
+// may not be finite. A tile that several groups' products read is zeroed by each of them: the same zeros, whenever the
+// others' products read them.
 __device__ __forceinline__ void zero_rows(uint8_t* at, int block, int blocks, int valid, int rows) {
     for (int i = threadIdx.x & 31; i < (rows - valid) * 8 * blocks; i += 32) {
         const int c = i & 7, b = (i >> 3) % blocks, r = valid + (i >> 3) / blocks;

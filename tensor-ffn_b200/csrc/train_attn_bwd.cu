@@ -8,7 +8,7 @@
 // The left products take both operands along the head from shared memory; the right ones take the streamed tile a second time, read the
 // other way round, and P or dS from the tensor memory that S or dP came from.
 //
-// D. rowsum(dO o O) with O as it was stored is off by 2^-9 of each term, and where a row sees few keys dP - D cancels: two keys of which
+// D. rowsum(dO o O) with O as it was stored is off by up to 2^-8 of each term, and where a row sees few keys dP - D cancels: two keys of which
 // one has all the weight leave 3% in dQ. So k<DQ> starts from that D', sums dS' = P o (dP - D') over the row in fp32, which is D - D', and
 // takes dQ = scale (sum dS' K - (D - D') sum P K); the exact D goes back to memory for k<DKV>. It costs the product P K, a fourth one.
 //
@@ -26,10 +26,11 @@
 // is what such a call waits for (32 ragged sequences of up to 512 queries, 14 / 2 heads of 64 columns: 112 us; with a variant of P for masks and
 // unrolled waits 157 us, and then with the results in the groups' hands 152 us).
 //
-// What bounds it: 128 columns: the products, 1 280 cycles a tile (1 x 8 192, 28 / 4 heads: 1 350 us, 0.89 PFLOP/s counted as the five products that
-// there have to be, 1.4 as the eight that are formed, under the power limit); 64 columns: 640 cycles of products, 512 of exponentials and
-// as many of fp32 arithmetic in about 900 (8 x 4 096, 14 / 2 heads: 856 us, 0.70); short sequences: the chain S, P, dP, dS, product of a unit of few
-// tiles, and the calls around (the 32 sequences above, with the order of units of now and all heads of a kv head in one block: 73 us, of which dot products 10).
+// What bounds it: 128 columns: the products, 1 280 cycles a tile, of which the left ones wait for shared memory, where both of their operands are
+// (1 x 8 192, 28 / 4 heads: 1 640 us in a row of calls, 0.74 PFLOP/s counted as the five products that there have to be, 1.2 as the eight that are
+// formed, under the power limit; 1 430 to 1 500 in calls by the dozen with pauses between); 64 columns: 640 cycles of products, 512 of exponentials and
+// as many of fp32 arithmetic in about 900 (8 x 4 096, 14 / 2 heads: 890 us, 0.68; in a row of calls 1 040); short sequences: the chain S, P, dP, dS, product of a unit of few
+// tiles, and the calls around (the 32 sequences above, with the order of units of now and all heads of a kv head in one block: 73 us, 77 on inputs that change from call to call, of which dot products 10).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cstring>
@@ -92,12 +93,12 @@ struct Cfg {
     static constexpr int BLOCK = kTile * 128, TILE = BLOCKS * BLOCK, STAGE = 2 * TILE;
     static constexpr int A_BLOCK = kStand * 128, A_TILE = BLOCKS * A_BLOCK, A_BYTES = 2 * A_TILE;
     static constexpr int UNITS = HD == 64 ? 2 : 1;                        // units whose standing rows are there: what 227 KB hold next to the ring
-    static constexpr int STAGES = HD == 64 ? 6 : 4;                       // at least two more than groups, for the loads on their way
+    static constexpr int STAGES = HD == 64 ? 6 : 4;                       // two more than groups at least, for the loads on their way
     static constexpr int RING = UNITS * A_BYTES, OUT = RING + STAGES * STAGE; // OUT: 2 KB a warp for results on their way out
     static constexpr int ROWS = OUT + 4 * 2048, ROWS_BYTES = GROUPS * 4 * 2 * kTile * 8;
     static constexpr int SLOTS = ROWS + ROWS_BYTES, BARS = SLOTS + kUnitSlots * (int)sizeof(Unit), SMEM = BARS + 448;
     static constexpr int ACC = GROUPS * 2 * kTile;                        // tensor memory: S and dP of each group, then two accumulators
-    static_assert(ACC + 2 * HD <= 512 && SMEM <= 227 * 1024 && STAGES > GROUPS && BARS % 8 == 0, "");
+    static_assert(ACC + 2 * HD <= 512 && SMEM <= 227 * 1024 && STAGES >= GROUPS + 2 && BARS % 8 == 0, "");
     static_assert(ROWS_BYTES >= 2 * GROUPS * kStand * 4, "");             // the groups' row sums of two units use the same place
 };
 

@@ -12,8 +12,8 @@
 // Bound by HBM: logits are read once and gradients written once. A row of a 151 936-word vocabulary is 608 KB, so a thread-block cluster
 // holds it in its shared memory between the sum and the gradient: each block one slice, fetched by bulk copies in pieces of 16 KB that
 // are summed as they land; the blocks exchange (maximum, sum, x[y]) through distributed shared memory. Slices of 76 KB leave three
-// blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 425 us,
-// 5.2 TB/s; blocks of 512 threads 434 us, and two of them an SM with slices of 108 KB 460 us; clusters of 14 with slices of 44 KB 454 us).
+// blocks an SM, so that one row's copies run under another's arithmetic and stores (2 048 rows of 151 936 fp32, a quarter of them masked: 428 us,
+// 5.1 TB/s; blocks of 512 threads 434 us, and two of them an SM with slices of 108 KB 460 us; clusters of 14 with slices of 44 KB 454 us).
 #include "launch.h"
 #include "pair.cuh"
 #include "ptx.cuh"
@@ -33,8 +33,8 @@ constexpr int kMaxBlocks = 8;              // blocks of a cluster
 constexpr int kMaxPieces = (kMaxSlice + kPiece - 1) / kPiece;
 constexpr int kHead = 256;                 // barriers and the blocks' partial results, in front of the slice
 
-// 2^x, x up to 0, on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by a polynomial of degree 6 fitted for the least largest relative error (1.9e-9, Remez
-// exchange), times 2^n; off by 7.7e-8 at most and not to one side. For the factors by which partial sums are joined: those of the exponential
+// 2^x, x up to 0, on the FMA pipe: x = n + f with |f| <= 1/2, 2^f by a polynomial of degree 6 fitted for the least largest relative error (Remez
+// exchange; 1.6e-8 with coefficients rounded to fp32), times 2^n; off by 7.9e-8 at most and not to one side. For the factors by which partial sums are joined: those of the exponential
 // unit are off to one side, ten of them in a row by 2.5e-7 (mean error of a log-probability over 32 768 words; with these 2e-8), and a KL term of a hundredth
 // multiplies that by fourteen. The single terms' errors average out; polynomials for them as well cost 18% of the time for nothing measurable.
 // 0 below -126, NaN of NaN.

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(block_of<TPR>(), Bwd<V, LAYER, TPR, N, L>::kPe
     __shared__ float slots[2][2][32];
     __shared__ uint64_t full[RING > 0 ? RING : 1];
     extern __shared__ __align__(128) uint8_t dynamic[];
-    float* const fold = (float*)dynamic;  // RPB > 1: [RPB - 1][width] sums of the other warps
+    float* const fold = (float*)dynamic;  // RPB > 1: [RPB][width] sums of the warps
     const int pitch = L == kShifted ? (width + 2 * V - 2) / V * V : width;
     T* const ring = (T*)dynamic;  // [RING][dy, x, skip][pitch], a row from the 16-byte unit on in which it begins
     pdl_launch_dependents();
