@@ -231,8 +231,8 @@ void* tffn_session_stream(const tffn_session* s);
  * CUDA graph (the first call of an operator on a device looks its kernels up and belongs outside of a capture), and leave the calling
  * thread's current device as it was. A workspace is the caller's and may be reused as soon as the stream has passed the call; calls
  * that can overlap, replayed graphs included, need workspaces of their own. Equal inputs give equal bits: no sum depends on timing.
- * Tensors start on a multiple of their element's size, or of what their call says. An output overlaps no other tensor of its call unless its comment says that it may be one of them. Arguments are checked before
- * anything is enqueued: TFFN_ERR_INVALID, TFFN_ERR_UNSUPPORTED. What only the device can
+ * Tensors start on a multiple of their element's size, or of what their call says. An output overlaps no other tensor of its call unless its
+ * comment says that it may be one of them. Arguments are checked before anything is enqueued: TFFN_ERR_INVALID, TFFN_ERR_UNSUPPORTED. What only the device can
  * see (a wait that ran out) is left in a status word per device: tffn_train_status. */
 enum { TFFN_DTYPE_BF16 = 0, TFFN_DTYPE_F32 = 1 };
 enum { TFFN_NORM_RMS = 0, TFFN_NORM_LAYER = 1 };

@@ -500,9 +500,9 @@ int run(AttnDev& p, const AttnCall& c, int num_sms, cudaStream_t s) {
     using C = Cfg<HD>;
     const int G = c.heads / c.kv_heads;
     const int64_t blocks = (c.max_q + kStand - 1) / kStand, all = blocks * c.n_seqs * c.heads;
-    // Units to themselves where every group of every SM gets four, counted by the bounds (ragged sequences have fewer: 32 x 512 2.6), us (one unit at a time against units of their own): 1 x 8 192, 28 heads of 128
-    // 467 against 411; 8 x 4 096, 14 heads of 64 390 against 319; 32 ragged x 512 of them 41 against 34; 3 x 2 777 of them in chunks of 1 024 44
-    // against 75; 1 x 1 000 of them 16 against 37.
+    // Units to themselves where every group of every SM gets four, counted by the bounds (ragged sequences have fewer: 32 x 512 2.6), us (one unit
+    // at a time against units of their own): 1 x 8 192, 28 heads of 128 467 against 411; 8 x 4 096, 14 heads of 64 390 against 319; 32 ragged x 512 of them
+    // 41 against 34; 3 x 2 777 of them in chunks of 1 024 44 against 75; 1 x 1 000 of them 16 against 37.
     p.parts = all <= 4 * C::GROUPS * num_sms ? 1 : C::GROUPS;
     const int64_t n = std::min<int64_t>(c.n_seqs, c.rows_q);  // sequences with rows
     const int64_t units = std::min((blocks * G + p.parts - 1) / p.parts * c.n_seqs, blocks_of_rows(c, c.max_q, c.rows_q) * G / p.parts + n) * c.kv_heads;

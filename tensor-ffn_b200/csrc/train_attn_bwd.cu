@@ -30,7 +30,8 @@
 // (1 x 8 192, 28 / 4 heads: 1 640 us in a row of calls, 0.74 PFLOP/s counted as the five products that there have to be, 1.2 as the eight that are
 // formed, under the power limit; 1 430 to 1 500 in calls by the dozen with pauses between); 64 columns: 640 cycles of products, 512 of exponentials and
 // as many of fp32 arithmetic in about 900 (8 x 4 096, 14 / 2 heads: 890 us, 0.68; in a row of calls 1 040); short sequences: the chain S, P, dP, dS, product of a unit of few
-// tiles, and the calls around (the 32 sequences above, with the order of units of now and all heads of a kv head in one block: 73 us, 77 on inputs that change from call to call, of which dot products 10).
+// tiles, and the calls around (the 32 sequences above, with the order of units of now and all heads of a kv head in one block: 73 us, of which dot
+// products 10; 77 on inputs that change from call to call).
 #include "train_attn.cuh"
 #include <algorithm>
 #include <cstring>
@@ -657,7 +658,8 @@ int run(AttnDev& p, int64_t units, int num_sms, cudaStream_t s, bool pdl) {
     using C = Cfg<HD>;
     const cudaError_t e = allow_shared<k_attn_bwd<HD, DKV>>(C::SMEM);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3(set_units(p, units, num_sms)), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
+    const unsigned grid = set_units(p, units, num_sms);
+    return (int)launch_k(k_attn_bwd<HD, DKV>, dim3(grid), dim3(C::THREADS), (size_t)C::SMEM, s, pdl, p);
 }
 
 // Parts of the query heads of a kv head for dK, dV. One block adds all of them up where there are one and a half units of work for each of the
